@@ -27,6 +27,16 @@ _c_int = ctypes.c_int
 _c_f32 = ctypes.c_float
 _vp = ctypes.c_void_p
 
+
+class Heads(ctypes.Structure):
+    """``dslpg_heads``: the layout that the rotary entry points share."""
+    _fields_ = ([(n, _c_i64) for n in ("batch", "seq", "q_heads", "k_heads", "head_dim", "rotary_dim")]
+                + [(n, _c_i64 * 3) for n in ("q_strides", "k_strides", "dq_strides", "dk_strides", "position_strides")]
+                + [("sections", _c_i64 * 4)]
+                + [(n, ctypes.c_int32) for n in ("axes", "interleaved", "dtype", "weight_dtype", "positions_dtype",
+                                                 "reserved")])
+
+
 # name -> argtypes (every entry point returns int)
 SIGNATURES = {
     "dslpg_layer_norm_fwd": [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _vp],
@@ -54,6 +64,11 @@ SIGNATURES = {
     "dslpg_rms_norm_fwd_host": [_vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _vp, _c_i64, _vp],
     "dslpg_layer_norm_fwd_host_workspace_bytes": [_c_i64, _c_i64, _c_int, _vp],
     "dslpg_layer_norm_fwd_host": [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _vp, _c_i64, _vp],
+    "dslpg_rope_fwd": [_vp] * 8,
+    "dslpg_rope_bwd": [_vp] * 8,
+    "dslpg_qk_norm_rope_fwd": [_vp] * 9 + [_c_f32, _vp],
+    "dslpg_qk_norm_rope_bwd_workspace_bytes": [_c_i64, _vp],
+    "dslpg_qk_norm_rope_bwd": [_vp] * 13 + [_c_f32, _vp, _c_i64, _vp],
     "dslpg_kernel_ff_static": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp],
     "dslpg_version": [],
     "dslpg_set_kernel_path": [_c_int],

@@ -262,6 +262,168 @@ py::object cross_entropy_fwd(py::handle logits_, py::handle labels_, py::handle 
   return py::make_tuple(loss, lse, z);
 }
 
+// A CUDA tensor of one of two dtypes on `dev`, else nullopt.
+std::optional<at::Tensor> cuda_of(const py::handle& h, int dev, at::ScalarType a, at::ScalarType b) {
+  if (!THPVariable_Check(h.ptr())) return std::nullopt;
+  const at::Tensor& t = THPVariable_Unpack(h.ptr());
+  if (!t.is_cuda() || t.get_device() != dev || (t.scalar_type() != a && t.scalar_type() != b)) return std::nullopt;
+  return t;
+}
+
+// Checked q and k with their layout (rope, qk_norm_rope).
+struct HeadRows {
+  at::Tensor q, k, pos, freq;
+  dslpg_heads h{};
+
+  static void strides(const at::Tensor& t, int64_t* out) {
+    const bool batched = t.dim() == 4;
+    out[0] = batched ? t.stride(0) : 0;
+    out[1] = t.stride(batched ? 1 : 0);
+    out[2] = t.stride(batched ? 2 : 1);
+  }
+
+  bool take(py::handle q_, py::handle k_, py::handle pos_, py::handle freq_, py::handle sections, py::handle inter) {
+    auto tq = cuda_float(q_);
+    if (!tq || (tq->dim() != 3 && tq->dim() != 4) || !PyBool_Check(inter.ptr())) return false;
+    const int dev = tq->get_device();
+    auto tk = cuda_float(k_, dev);
+    auto tp = cuda_of(pos_, dev, at::kLong, at::kInt);
+    auto tf = cuda_of(freq_, dev, at::kFloat, at::kFloat);
+    if (!tk || !tp || !tf || tk->scalar_type() != tq->scalar_type() || tk->dim() != tq->dim()) return false;
+    const int64_t nd = tq->dim(), lead = nd - 2, d = tq->size(-1);
+    for (int64_t i = 0; i < lead; ++i)
+      if (tk->size(i) != tq->size(i)) return false;
+    if (tq->numel() == 0 || tk->numel() == 0 || tk->size(-1) != d || d > 1024 || tq->stride(-1) != 1 ||
+        tk->stride(-1) != 1 || tf->dim() != 1 || tf->stride(0) != 1 || tf->size(0) < 1 || 2 * tf->size(0) > d ||
+        (tq->numel() + tk->numel()) / d > (1ll << 30))
+      return false;
+    h.axes = 1;
+    h.sections[0] = tf->size(0);
+    if (!sections.is_none()) {
+      if (!PyTuple_Check(sections.ptr()) && !PyList_Check(sections.ptr())) return false;
+      py::sequence seq = py::reinterpret_borrow<py::sequence>(sections);
+      if (seq.size() < 1 || seq.size() > 4) return false;
+      int64_t left = tf->size(0);
+      for (size_t i = 0; i < seq.size(); ++i) {
+        if (!is_int(seq[i])) return false;
+        h.sections[i] = seq[i].cast<int64_t>();
+        if (h.sections[i] < 0 || h.sections[i] > left) return false;
+        left -= h.sections[i];
+      }
+      if (left != 0) return false;
+      h.axes = static_cast<int32_t>(seq.size());
+    }
+    // positions: [axes,] tokens, or what broadcasts to that from the right
+    const int64_t want = lead + (sections.is_none() ? 0 : 1);
+    if (tp->dim() > want) return false;
+    int64_t ps[3] = {0, 0, 0};  // axis, batch, seq
+    for (int64_t i = 1; i <= tp->dim(); ++i) {
+      const int64_t extent = i <= lead ? tq->size(lead - i) : h.axes;
+      const int64_t size = tp->size(tp->dim() - i);
+      if (size != extent && size != 1) return false;
+      const int slot = i > lead ? 0 : (i == 1 ? 2 : 1);
+      ps[slot] = size == 1 ? 0 : tp->stride(tp->dim() - i);
+    }
+    for (int i = 0; i < 3; ++i) h.position_strides[i] = ps[i];
+    h.batch = lead == 2 ? tq->size(0) : 1;
+    h.seq = tq->size(lead - 1);
+    h.q_heads = tq->size(lead);
+    h.k_heads = tk->size(lead);
+    h.head_dim = d;
+    h.rotary_dim = 2 * tf->size(0);
+    strides(*tq, h.q_strides);
+    strides(*tk, h.k_strides);
+    h.interleaved = inter.ptr() == Py_True ? 1 : 0;
+    h.dtype = float_code(tq->scalar_type());
+    h.positions_dtype = tp->scalar_type() == at::kLong ? DSLPG_I64 : DSLPG_I32;
+    q = *tq;
+    k = *tk;
+    pos = *tp;
+    freq = *tf;
+    return true;
+  }
+
+  // The norm weights: [head_dim] vectors of one float dtype.
+  bool weights(py::handle qw_, py::handle kw_, at::Tensor& qw, at::Tensor& kw) {
+    auto a = cuda_float(qw_, q.get_device()), b = cuda_float(kw_, q.get_device());
+    if (!a || !b || a->scalar_type() != b->scalar_type() || a->dim() != 1 || b->dim() != 1 ||
+        a->size(0) != h.head_dim || b->size(0) != h.head_dim || !a->is_contiguous() || !b->is_contiguous())
+      return false;
+    h.weight_dtype = float_code(a->scalar_type());
+    qw = *a;
+    kw = *b;
+    return true;
+  }
+
+  at::Tensor dense(const at::Tensor& t) const { return at::empty(t.sizes(), t.options()); }
+};
+
+py::object rotate(bool bwd, py::handle q, py::handle k, py::handle pos, py::handle freq, py::handle sections,
+                  py::handle inter) {
+  HeadRows r;
+  if (!r.take(q, k, pos, freq, sections, inter)) return py::none();
+  at::Tensor yq = r.dense(r.q), yk = r.dense(r.k);
+  launch(r.q, bwd ? "dslpg_rope_bwd" : "dslpg_rope_fwd", [&](cudaStream_t s) {
+    return (bwd ? dslpg_rope_bwd : dslpg_rope_fwd)(r.q.data_ptr(), r.k.data_ptr(), r.pos.data_ptr(),
+                                                   r.freq.data_ptr<float>(), yq.data_ptr(), yk.data_ptr(), &r.h, s);
+  });
+  return py::make_tuple(yq, yk);
+}
+
+py::object rope(py::handle q, py::handle k, py::handle pos, py::handle freq, py::handle sections, py::handle inter) {
+  return rotate(false, q, k, pos, freq, sections, inter);
+}
+
+py::object rope_bwd(py::handle q, py::handle k, py::handle pos, py::handle freq, py::handle sections,
+                    py::handle inter) {
+  return rotate(true, q, k, pos, freq, sections, inter);
+}
+
+py::object qk_norm_rope(py::handle q, py::handle k, py::handle qw_, py::handle kw_, py::handle pos, py::handle freq,
+                        py::handle eps, py::handle sections, py::handle inter) {
+  HeadRows r;
+  at::Tensor qw, kw;
+  if (!(PyFloat_Check(eps.ptr()) || is_int(eps)) || !r.take(q, k, pos, freq, sections, inter) ||
+      !r.weights(qw_, kw_, qw, kw))
+    return py::none();
+  at::Tensor yq = r.dense(r.q), yk = r.dense(r.k);
+  launch(r.q, "dslpg_qk_norm_rope_fwd", [&](cudaStream_t s) {
+    return dslpg_qk_norm_rope_fwd(r.q.data_ptr(), r.k.data_ptr(), qw.data_ptr(), kw.data_ptr(), r.pos.data_ptr(),
+                                  r.freq.data_ptr<float>(), yq.data_ptr(), yk.data_ptr(), &r.h,
+                                  static_cast<float>(eps.cast<double>()), s);
+  });
+  return py::make_tuple(yq, yk);
+}
+
+py::object qk_norm_rope_bwd(py::handle dq_, py::handle dk_, py::handle q, py::handle k, py::handle qw_,
+                            py::handle kw_, py::handle pos, py::handle freq, py::handle eps, py::handle sections,
+                            py::handle inter) {
+  HeadRows r;
+  at::Tensor qw, kw;
+  if (!(PyFloat_Check(eps.ptr()) || is_int(eps)) || !r.take(q, k, pos, freq, sections, inter) ||
+      !r.weights(qw_, kw_, qw, kw))
+    return py::none();
+  auto gq = cuda_float(dq_, r.q.get_device()), gk = cuda_float(dk_, r.q.get_device());
+  if (!gq || !gk || gq->scalar_type() != r.q.scalar_type() || gk->scalar_type() != r.q.scalar_type() ||
+      gq->sizes() != r.q.sizes() || gk->sizes() != r.k.sizes() || gq->stride(-1) != 1 || gk->stride(-1) != 1)
+    return py::none();
+  HeadRows::strides(*gq, r.h.dq_strides);
+  HeadRows::strides(*gk, r.h.dk_strides);
+  at::Tensor dq = r.dense(r.q), dk = r.dense(r.k);
+  const auto f32 = r.q.options().dtype(at::kFloat);
+  at::Tensor dqw = at::empty({r.h.head_dim}, f32), dkw = at::empty({r.h.head_dim}, f32);
+  int64_t need = 0;
+  if (dslpg_qk_norm_rope_bwd_workspace_bytes(r.h.head_dim, &need) != 0) return py::none();
+  at::Tensor ws = at::empty({need}, r.q.options().dtype(at::kByte));
+  launch(r.q, "dslpg_qk_norm_rope_bwd", [&](cudaStream_t s) {
+    return dslpg_qk_norm_rope_bwd(gq->data_ptr(), gk->data_ptr(), r.q.data_ptr(), r.k.data_ptr(), qw.data_ptr(),
+                                  kw.data_ptr(), r.pos.data_ptr(), r.freq.data_ptr<float>(), dq.data_ptr(),
+                                  dk.data_ptr(), dqw.data_ptr<float>(), dkw.data_ptr<float>(), &r.h,
+                                  static_cast<float>(eps.cast<double>()), ws.data_ptr(), need, s);
+  });
+  return py::make_tuple(dq, dk, dqw, dkw);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dslpg_torch, m) {
@@ -275,4 +437,8 @@ PYBIND11_MODULE(_dslpg_torch, m) {
   m.def("max_reduction", &max_reduction);
   m.def("argmax", &argmax);
   m.def("cross_entropy_fwd", &cross_entropy_fwd);
+  m.def("rope", &rope);
+  m.def("rope_bwd", &rope_bwd);
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd);
 }

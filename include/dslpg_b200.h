@@ -303,6 +303,63 @@ DSLPG_API int dslpg_kernel_ff(const void* x, const void* w1, const void* w3, con
 DSLPG_API int dslpg_kernel_ff_static(const void* x, const void* w1, const void* w3, const void* rms_w, void* out,
                                      int64_t M, int64_t N, int64_t K, cudaStream_t stream);
 
+/*
+ * Per-head RMSNorm with the rotary position rotation, and the rotation alone,
+ * forward and backward.
+ *
+ * q is [batch, seq, q_heads, head_dim] and k [batch, seq, k_heads, head_dim],
+ * each with its own batch, seq and head strides (in elements; the last axis is
+ * dense), so both may be views into one projection output. Outputs are dense
+ * in that order. With n = rotary_dim / 2 frequencies inv_freq[i] (float32),
+ * phi_i = position * inv_freq[i], and pairs (i, i + n) (or (2i, 2i + 1) when
+ * `interleaved`) of the first rotary_dim features:
+ *   u = x / sqrt(mean(x^2) + eps) * weight            (rope: u = x)
+ *   y_i = u_i cos phi_i - u_j sin phi_i;   y_j = u_j cos phi_i + u_i sin phi_i
+ * and the features past rotary_dim are u. Arithmetic is fp32 with one rounding
+ * at the store; the angles are formed in 64 bits, so that far positions keep
+ * the cosine to fp32 accuracy.
+ *
+ * `positions` (int32 or int64) has `axes` (1 to 4) values for each token, with
+ * axis, batch and seq strides (0: broadcast). Frequency i turns by axis a where
+ * sections[0] + ... + sections[a - 1] <= i < sections[0] + ... + sections[a];
+ * the sections add up to n.
+ *
+ * head_dim is at most 1024, and batch * seq * (q_heads + k_heads) at most 2^30.
+ * q's pointers may be NULL when q_heads is 0, and k's when k_heads is 0.
+ * No reference counterpart: the suite has the norm (rms_norm), not this form.
+ */
+typedef struct dslpg_heads {
+  int64_t batch, seq, q_heads, k_heads, head_dim, rotary_dim;
+  int64_t q_strides[3], k_strides[3];    /* batch, seq, head; rope_bwd: of dq_out and dk_out */
+  int64_t dq_strides[3], dk_strides[3];  /* qk_norm_rope_bwd: of dq_out and dk_out */
+  int64_t position_strides[3];           /* axis, batch, seq */
+  int64_t sections[4];                   /* the first `axes` of them */
+  int32_t axes, interleaved;
+  int32_t dtype, weight_dtype, positions_dtype; /* q and k; both weights; I32 or I64 */
+  int32_t reserved;
+} dslpg_heads;
+
+DSLPG_API int dslpg_rope_fwd(const void* q, const void* k, const void* positions, const float* inv_freq, void* q_out,
+                             void* k_out, const dslpg_heads* heads, cudaStream_t stream);
+
+/* The rotation by -phi: the gradients of rope_fwd's inputs. */
+DSLPG_API int dslpg_rope_bwd(const void* dq_out, const void* dk_out, const void* positions, const float* inv_freq,
+                             void* dq, void* dk, const dslpg_heads* heads, cudaStream_t stream);
+
+DSLPG_API int dslpg_qk_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                     const void* positions, const float* inv_freq, void* q_out, void* k_out,
+                                     const dslpg_heads* heads, float eps, cudaStream_t stream);
+
+/* dq, dk (dense, q's type) and the weights' gradients (float32, [head_dim],
+ * summed over all tokens and heads in a fixed order). `workspace` (16-byte
+ * aligned): dslpg_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes. */
+DSLPG_API int dslpg_qk_norm_rope_bwd_workspace_bytes(int64_t head_dim, int64_t* bytes);
+DSLPG_API int dslpg_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                     const void* q_weight, const void* k_weight, const void* positions,
+                                     const float* inv_freq, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                                     const dslpg_heads* heads, float eps, void* workspace, int64_t workspace_bytes,
+                                     cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
