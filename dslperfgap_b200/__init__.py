@@ -17,6 +17,9 @@ from .argmax.cuda_impl import argmax
 from .linear_activation.cuda_impl import kernel_ff
 from .qk_norm_rope.cuda_impl import qk_norm_rope, qk_norm_rope_bwd
 from .rope.cuda_impl import rope, rope_bwd
+from .policy_loss.cuda_impl import policy_loss_fwd, policy_loss_bwd, policy_loss_fwd_bwd
+from .preference_loss.cuda_impl import preference_loss_fwd, preference_loss_bwd
 
 __all__ = ["layer_norm", "layer_norm_host", "rms_norm", "rms_norm_host", "softmax", "log_softmax", "logsumexp", "cross_entropy_fwd", "cross_entropy_bwd", "cross_entropy_fwd_bwd",
-           "mean_reduction", "max_reduction", "argmax", "kernel_ff", "qk_norm_rope", "qk_norm_rope_bwd", "rope", "rope_bwd"]
+           "mean_reduction", "max_reduction", "argmax", "kernel_ff", "qk_norm_rope", "qk_norm_rope_bwd", "rope", "rope_bwd",
+           "policy_loss_fwd", "policy_loss_bwd", "policy_loss_fwd_bwd", "preference_loss_fwd", "preference_loss_bwd"]

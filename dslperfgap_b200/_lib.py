@@ -37,6 +37,27 @@ class Heads(ctypes.Structure):
                                                  "reserved")])
 
 
+class LogitRows(ctypes.Structure):
+    """``dslpg_logit_rows``: the logits and labels of a loss."""
+    _fields_ = ([("logits", _vp), ("labels", _vp)]
+                + [(n, _c_i64) for n in ("n_rows", "n_cols", "row_stride", "ignored_index")]
+                + [("logit_scale", ctypes.c_double), ("logits_dtype", ctypes.c_int32), ("labels_dtype", ctypes.c_int32)])
+
+
+class PolicyTerms(ctypes.Structure):
+    """``dslpg_policy_terms``: what the policy loss takes per row."""
+    _fields_ = ([(n, _vp) for n in ("old_logp", "advantages", "ref_logp")]
+                + [(n, _c_i64) for n in ("old_stride", "advantages_stride", "ref_stride")]
+                + [(n, _c_f32) for n in ("clip_low", "clip_high", "kl_coef", "reserved")])
+
+
+class PairTerms(ctypes.Structure):
+    """``dslpg_pair_terms``: the sequences of the preference loss."""
+    _fields_ = ([("seq_starts", _vp), ("ref_logp", _vp), ("n_pairs", _c_i64), ("ref_stride", _c_i64),
+                 ("beta", _c_f32), ("smoothing", _c_f32), ("starts_dtype", ctypes.c_int32),
+                 ("reserved", ctypes.c_int32)])
+
+
 # name -> argtypes (every entry point returns int)
 SIGNATURES = {
     "dslpg_layer_norm_fwd": [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _vp],
@@ -69,6 +90,11 @@ SIGNATURES = {
     "dslpg_qk_norm_rope_fwd": [_vp] * 9 + [_c_f32, _vp],
     "dslpg_qk_norm_rope_bwd_workspace_bytes": [_c_i64, _vp],
     "dslpg_qk_norm_rope_bwd": [_vp] * 13 + [_c_f32, _vp, _c_i64, _vp],
+    "dslpg_policy_loss_fwd": [_vp] * 7,
+    "dslpg_policy_loss_bwd": [_vp, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _vp],
+    "dslpg_policy_loss_fwd_bwd": [_vp, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _vp],
+    "dslpg_preference_loss_fwd": [_vp] * 7,
+    "dslpg_preference_loss_bwd": [_vp, _vp, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _vp],
     "dslpg_kernel_ff_static": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp],
     "dslpg_version": [],
     "dslpg_set_kernel_path": [_c_int],

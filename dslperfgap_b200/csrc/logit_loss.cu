@@ -1,0 +1,681 @@
+// logit_loss.cu — losses of post-training on rows of logits and their
+// gradients (sm_100a): the clipped policy loss with a KL term and the
+// preference loss on paired sequences.
+//
+// For a row with scaled logits z = scale * x and label y:
+//   lse = log sum exp z,  logp = z_y - lse.
+// Policy: r = exp(logp - old), l1 = -r A, l2 = -clip(r, lo, hi) A, d = ref - logp,
+//   kl = exp(d) - d - 1,  loss = max(l1, l2) + beta kl,
+//   g = dloss/dlogp = (l2 > l1 ? 0 : -r A) + beta (1 - exp(d)).
+// Preference: S_s = sum over the sequence's rows of logp - ref, m = beta (S_chosen - S_rejected),
+//   loss = (1 - e) softplus(-m) + e softplus(m),
+//   g = +-beta (e sigmoid(m) - (1 - e) sigmoid(-m)) on the chosen / rejected rows.
+// Both: dlogits[c] = dloss g scale ([c == y] - exp(z_c - lse)).
+//
+// A row is left out when its label is the ignored index or no column (and, for
+// preferences, when it lies in no sequence): its logits are not read, its
+// results and gradients are 0.
+//
+// Statistics: d = (x - m) scale log2(e) against the running extreme m (the
+// largest x, or the smallest for a negative scale), an online sum of 2^d per
+// thread; then logp = scale (x_y - m) - ln s and lse = scale m + ln s, in 64 bits
+// once per row. x - m is 0 at the extreme whatever its size, so a row masked
+// with the type's lowest value throughout is a uniform row. The constant has two
+// float32 parts: rounded to one it would shift every lse of a call in the same
+// direction (some 2e-7), which a sum over a sequence's rows adds up. Both parts
+// have one sign, so that a logit of -inf gives d = -inf and not NaN.
+#include "common.cuh"
+
+namespace dslpg {
+
+struct LossRows {
+  const void* x;
+  const void* labels;
+  int64_t M, N, ld, ignored;
+  int label64;
+  double scale;
+  float scale_f, sign;  // scale as float32; 1 or -1
+  float c_hi, c_lo;     // scale * log2(e) in two parts of one sign
+  int tpr, rpc;         // threads of a row, rows of a CTA (statistics kernel)
+  int nvec;             // N / V on the vector path
+};
+
+struct PolicyTerms {
+  const float *old_logp, *adv, *ref;
+  int64_t old_stride, adv_stride, ref_stride;
+  float lo, hi, kl_coef;
+};
+
+struct PairTerms {
+  const void* starts;
+  int starts64;
+  int64_t pairs;
+  const float* ref;
+  int64_t ref_stride;
+  float beta, smoothing;
+};
+
+struct LossOut {
+  float *loss, *logp, *lse, *kl;
+};
+
+struct GradOut {
+  const float* dloss;
+  int64_t dloss_stride;
+  const float* lse;        // backward: the forward's
+  const float* log_ratio;  // preference backward
+  void* dx;
+  int64_t ldo;
+};
+
+// Sequence bound s of a preference batch, kept inside the rows.
+DSLPG_DEV int64_t start_at(const PairTerms& p, int64_t s, int64_t rows) {
+  const int64_t v = p.starts64 ? static_cast<const int64_t*>(p.starts)[s]
+                               : static_cast<int64_t>(static_cast<const int32_t*>(p.starts)[s]);
+  return v < 0 ? 0 : (v > rows ? rows : v);
+}
+
+// Column of row r's label, or -1 when the row is left out.
+DSLPG_DEV int64_t label_col(const LossRows& a, int64_t r) {
+  const int64_t y = a.label64 ? static_cast<const int64_t*>(a.labels)[r]
+                              : static_cast<int64_t>(static_cast<const int32_t*>(a.labels)[r]);
+  return (y == a.ignored || y < 0 || y >= a.N) ? -1 : y;
+}
+
+// The row's sequence (the last one that starts at or before r), or -1 outside all of them.
+DSLPG_DEV int64_t sequence_of(const PairTerms& p, int64_t r, int64_t rows) {
+  const int64_t n = 2 * p.pairs;
+  if (r < start_at(p, 0, rows) || r >= start_at(p, n, rows)) return -1;
+  int64_t lo = 0, hi = n;  // starts[lo] <= r < starts[hi]
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (start_at(p, mid, rows) <= r) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Online statistics of one thread: m = the largest sign * x, s = the sum of
+// 2^((sign x - m) |c|).
+struct Stat {
+  float m = kNegInf, s = 0.f;
+  DSLPG_DEV void rebase(float nm, const LossRows& a) {
+    if (m != nm && m != kNegInf) s *= ex2((m - nm) * fabsf(a.c_hi));  // s is 0 while m = -inf
+    m = nm;
+  }
+};
+
+// n logits, of which those with ok[i] count.
+template <int n> DSLPG_DEV void fold_values(Stat& st, const float (&x)[n], const bool (&ok)[n], const LossRows& a) {
+  float nm = st.m;
+#pragma unroll
+  for (int i = 0; i < n; ++i)
+    if (ok[i]) nm = max_nan(nm, x[i] * a.sign);
+  if (nm == kNegInf) return;  // nothing but -inf so far
+  st.rebase(nm, a);
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const float y = x[i] - nm * a.sign;
+    if (ok[i]) st.s += ex2(fmaf(y, a.c_lo, y * a.c_hi));
+  }
+}
+
+// NV vectors of logits, all valid.
+template <typename T, int NV>
+DSLPG_DEV void fold_rows(Stat& st, const Vec16 (&v)[NV], const LossRows& a) {
+  constexpr int P = Elt<T>::kPerVec / 2;
+  const float ext = (a.sign >= 0.f) ? RawExtreme<T, NV, false>::run(v) : RawExtreme<T, NV, true>::run(v);
+  const float nm = max_nan(st.m, ext * a.sign);
+  if (nm == kNegInf) return;
+  const f32x2 hi = pk2(a.c_hi, a.c_hi), lo = pk2(a.c_lo, a.c_lo), neg = pk2(-nm * a.sign, -nm * a.sign);
+  f32x2 acc[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const f32x2 y = add2(unpack_pair<T>(v[k], p), neg);
+      float d0, d1;
+      upk2(fma2(y, lo, mul2(y, hi)), d0, d1);
+      acc[p & 1] = add2(acc[p & 1], pk2(ex2(d0), ex2(d1)));
+    }
+  st.rebase(nm, a);
+  st.s += hsum2(add2(acc[0], acc[1]));
+}
+
+// A thread's sum against the row's extreme.
+DSLPG_DEV float merged(const Stat& st, float gm, const LossRows& a) {
+  return (st.m == gm || st.m == kNegInf) ? st.s : st.s * ex2((st.m - gm) * fabsf(a.c_hi));
+}
+
+// A row's merged statistics. Where the extreme is not finite, all of it is NaN.
+struct RowStat {
+  float m, log2s;  // the extreme x itself; log2 of the sum
+  DSLPG_DEV RowStat(float gm, float gs, const LossRows& a)
+      : m(gm * a.sign), log2s(fabsf(gm) < kPosInf ? log2f(gs) : __builtin_nanf("")) {}
+  DSLPG_DEV double ln_s() const { return 0.69314718055994530942 * static_cast<double>(log2s); }
+  DSLPG_DEV double lse(const LossRows& a) const { return a.scale * static_cast<double>(m) + ln_s(); }
+  DSLPG_DEV double logp(const LossRows& a, float xl) const {
+    return a.scale * (static_cast<double>(xl) - static_cast<double>(m)) - ln_s();
+  }
+};
+
+struct PolicyRow {
+  float loss, kl, g;  // g: dloss / dlogp
+};
+
+DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, int64_t r, double logp) {
+  const float adv = p.adv[r * p.adv_stride];
+  const float ratio = expf(static_cast<float>(logp - static_cast<double>(p.old_logp[r * p.old_stride])));
+  const float l1 = -ratio * adv, l2 = -fminf(fmaxf(ratio, p.lo), p.hi) * adv;
+  PolicyRow o{max_nan(l1, l2), 0.f, l2 > l1 ? 0.f : l1};
+  if (p.ref != nullptr) {
+    const float d = static_cast<float>(static_cast<double>(p.ref[r * p.ref_stride]) - logp);
+    const float e = expm1f(d);
+    // exp(d) - d - 1; its power series near 0, where the difference cancels (|d| < 1/4: the first term left out is
+    // below 2e-8 of the sum)
+    o.kl = fabsf(d) < 0.25f
+               ? d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040))))))
+               : e - d;
+    if (p.kl_coef != 0.f) {
+      o.loss += p.kl_coef * o.kl;
+      o.g -= p.kl_coef * e;
+    }
+  }
+  return o;
+}
+
+// dloss g of a preference row in sequence `seq` (chosen ones first).
+DSLPG_DEV float pair_slope(const PairTerms& p, const float* log_ratio, int64_t seq) {
+  const bool chosen = seq < p.pairs;
+  const int64_t k = chosen ? seq : seq - p.pairs;
+  const float m = p.beta * (log_ratio[k] - log_ratio[p.pairs + k]);
+  const float up = 1.f / (1.f + expf(-m)), down = 1.f / (1.f + expf(m));  // sigmoid(m), sigmoid(-m)
+  const float slope = p.beta * (p.smoothing * up - (1.f - p.smoothing) * down);
+  return chosen ? slope : -slope;
+}
+
+enum LossKind : int { kPolicy = 0, kPair = 1 };
+
+// Fold a whole row with `tpr` threads, this one being t: 16-byte vectors
+// (V > 1), the next ones loaded before this round's arithmetic, or scalars.
+template <typename T, int V, int U, class Load>
+DSLPG_DEV void fold_row(Stat& st, const T* xr, const LossRows& a, int t, int tpr, Load ld) {
+  if constexpr (V > 1) {
+    const int stride = U * tpr;
+    auto load = [&](Vec16 (&dst)[U], int j0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * tpr;
+        dst[u] = Vec16{{0u, 0u, 0u, 0u}};
+        if (j < a.nvec) dst[u] = ld(xr + static_cast<int64_t>(j) * V);
+      }
+    };
+    Vec16 nx[U];
+    load(nx, t);
+    for (int j0 = t; j0 < a.nvec; j0 += stride) {
+      Vec16 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = nx[u];
+      if (j0 + stride < a.nvec) load(nx, j0 + stride);
+      if (j0 + (U - 1) * tpr < a.nvec) {
+        fold_rows<T, U>(st, v, a);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (j0 + u * tpr < a.nvec) {
+            const Vec16 one[1] = {v[u]};
+            fold_rows<T, 1>(st, one, a);
+          }
+        }
+      }
+    }
+  } else {
+    constexpr int W = 8;
+    for (int64_t j0 = t; j0 < a.N; j0 += static_cast<int64_t>(W) * tpr) {
+      float x[W];
+      bool ok[W];
+#pragma unroll
+      for (int u = 0; u < W; ++u) {
+        const int64_t j = j0 + static_cast<int64_t>(u) * tpr;
+        ok[u] = j < a.N;
+        x[u] = ok[u] ? to_f(xr[j]) : 0.f;
+      }
+      fold_values<W>(st, x, ok, a);
+    }
+  }
+}
+
+// Row statistics: `tpr` threads a row. Writes the row's losses (policy) or its
+// logp and lse (preferences; pair_kernel then sums them).
+template <int KIND, typename T, int V>
+__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const LossRows a, const PolicyTerms pol, const PairTerms pair,
+                                                           const LossOut o) {
+  __shared__ float red[2][32];
+  const int g = threadIdx.x / a.tpr, t = threadIdx.x - g * a.tpr;
+  const int nw = a.tpr >> 5, first_warp = g * nw;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.rpc; base < a.M; base += step) {
+    const int64_t r = base + g;
+    int64_t col = r < a.M ? label_col(a, r) : -1;
+    if constexpr (KIND == kPair)
+      if (col >= 0 && sequence_of(pair, r, a.M) < 0) col = -1;
+    const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+    Stat st;
+    float xl = 0.f;
+    if (col >= 0) {
+      if (t == 0) xl = to_f(xr[col]);
+      fold_row<T, V, 4>(st, xr, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+    }
+    const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
+    const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
+    if (t == 0 && r < a.M) {
+      double logp = 0.0, lse = 0.0;
+      PolicyRow p{0.f, 0.f, 0.f};
+      if (col >= 0) {
+        const RowStat rs(gm, gs, a);
+        lse = rs.lse(a);
+        logp = rs.logp(a, xl);
+        if constexpr (KIND == kPolicy) p = policy_row(pol, r, logp);
+      }
+      o.logp[r] = static_cast<float>(logp);
+      o.lse[r] = static_cast<float>(lse);
+      if constexpr (KIND == kPolicy) {
+        o.loss[r] = p.loss;
+        o.kl[r] = p.kl;
+      }
+    }
+  }
+}
+
+DSLPG_DEV double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+
+// One CTA a pair: the two sequences' sums of logp - ref (64 bits, in a fixed
+// order), their margin and the pair's loss.
+__global__ void __launch_bounds__(256) pair_kernel(const LossRows a, const PairTerms p, const float* logp, float* loss,
+                                                   float* log_ratio) {
+  __shared__ double part[2][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t k = blockIdx.x; k < p.pairs; k += gridDim.x) {
+    for (int side = 0; side < 2; ++side) {
+      const int64_t s = k + side * p.pairs;
+      const int64_t lo = start_at(p, s, a.M), hi = start_at(p, s + 1, a.M);
+      double sum = 0.0;
+      for (int64_t r = lo + threadIdx.x; r < hi; r += blockDim.x)
+        if (label_col(a, r) >= 0) sum += static_cast<double>(logp[r]) - static_cast<double>(p.ref[r * p.ref_stride]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) part[side][warp] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double t[2] = {0.0, 0.0};
+      for (int side = 0; side < 2; ++side) {
+        for (int w = 0; w < 8; ++w) t[side] += part[side][w];
+        log_ratio[k + side * p.pairs] = static_cast<float>(t[side]);
+      }
+      const double m = static_cast<double>(p.beta) * (t[0] - t[1]), e = p.smoothing;
+      // a term of weight 0 is left out: an infinite margin would make it NaN
+      const double up = e < 1.0 ? (1.0 - e) * softplus(-m) : 0.0, down = e > 0.0 ? e * softplus(m) : 0.0;
+      loss[k] = static_cast<float>(up + down);
+    }
+    __syncthreads();
+  }
+}
+
+// dlogits[c] = k1 2^((x + shift) c + off), with k1 = -dloss g scale.
+struct GradTerms {
+  float k1, shift, c, off;
+};
+
+// dlogits of one row by `nt` threads, then the label column, k1 expm1(logp).
+// The next chunk's loads are issued before this chunk's arithmetic.
+template <typename T, int V, int U>
+DSLPG_DEV void grad_row(const T* xr, T* yr, const LossRows& a, const GradTerms& gt, double logp, int64_t col, int t,
+                        int nt) {
+  if constexpr (V > 1) {
+    constexpr int P = Elt<T>::kPerVec / 2;
+    auto load = [&](Vec16 (&dst)[U], int j0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * nt;
+        dst[u] = Vec16{{0u, 0u, 0u, 0u}};
+        if (j < a.nvec) dst[u] = ld_stream(xr + static_cast<int64_t>(j) * V);
+      }
+    };
+    const f32x2 c2 = pk2(gt.c, gt.c), sh2 = pk2(gt.shift, gt.shift), off2 = pk2(gt.off, gt.off), k2 = pk2(gt.k1, gt.k1);
+    Vec16 nx[U];
+    load(nx, t);
+    for (int j0 = t; j0 < a.nvec; j0 += U * nt) {
+      Vec16 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = nx[u];
+      if (j0 + U * nt < a.nvec) load(nx, j0 + U * nt);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * nt;
+        if (j >= a.nvec) continue;
+        f32x2 y[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          float d0, d1;
+          upk2(fma2(add2(unpack_pair<T>(v[u], p), sh2), c2, off2), d0, d1);
+          y[p] = mul2(k2, pk2(ex2(d0), ex2(d1)));
+        }
+        StorePairs<T, P>::run(yr + static_cast<int64_t>(j) * V, y);
+      }
+    }
+  } else {
+    for (int64_t j = t; j < a.N; j += nt) yr[j] = from_f<T>(gt.k1 * ex2(fmaf(to_f(xr[j]) + gt.shift, gt.c, gt.off)));
+  }
+  // the label column, rewritten by the thread that wrote its vector or element
+  const int64_t unit = V > 1 ? col / V : col;
+  if (static_cast<int>(unit % nt) == t) yr[col] = from_f<T>(gt.k1 * expm1f(static_cast<float>(logp)));
+}
+
+template <typename T, int V> DSLPG_DEV void zero_row(T* yr, const LossRows& a, int t, int nt) {
+  if constexpr (V > 1) {
+    for (int j = t; j < a.nvec; j += nt) st_stream(yr + static_cast<int64_t>(j) * V, Vec16{{0u, 0u, 0u, 0u}});
+  } else {
+    for (int64_t j = t; j < a.N; j += nt) yr[j] = from_f<T>(0.f);
+  }
+}
+
+// Beyond this a float32 lse no longer tells the row's probabilities to 2e-5 (a
+// row masked with the type's lowest value throughout has lse = -3e38 + ln N).
+constexpr float kLseTrusted = 256.f;
+
+// The gradient alone, from the forward's lse: a CTA a row, read once and written
+// once. Rows whose lse is beyond kLseTrusted have their statistics formed again.
+template <int KIND, typename T, int V>
+__global__ void __launch_bounds__(256) loss_bwd_kernel(const LossRows a, const PolicyTerms pol, const PairTerms pair,
+                                                       const GradOut o) {
+  __shared__ float red[2][32];
+  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
+    T* yr = static_cast<T*>(o.dx) + r * o.ldo;
+    const int64_t col = label_col(a, r);
+    int64_t seq = 0;
+    if (KIND == kPair && col >= 0) seq = sequence_of(pair, r, a.M);
+    if (col < 0 || seq < 0) {
+      zero_row<T, V>(yr, a, threadIdx.x, blockDim.x);
+      continue;
+    }
+    const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+    const float lse = o.lse[r], xl = to_f(xr[col]);
+    double logp = static_cast<double>(xl) * a.scale - static_cast<double>(lse);
+    // p = 2^((x - lse / scale) c); at scale 0 the row is uniform
+    GradTerms gt{0.f, 0.f, a.c_hi, -lse * kLog2e};
+    if (a.scale != 0.0) {
+      gt.shift = -static_cast<float>(static_cast<double>(lse) / a.scale);
+      gt.off = 0.f;
+    }
+    if (!(fabsf(lse) <= kLseTrusted)) {
+      Stat st;
+      fold_row<T, V, 1>(st, xr, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
+      const int nw = blockDim.x >> 5;
+      const float gm = group_reduce<MaxOp>(st.m, red[0], nw, 0);
+      const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, 0);
+      const RowStat rs(gm, gs, a);
+      logp = rs.logp(a, xl);
+      gt.shift = -rs.m;
+      gt.off = -rs.log2s;
+    }
+    float g, dl;
+    if constexpr (KIND == kPolicy) {
+      g = policy_row(pol, r, logp).g;
+      dl = o.dloss[r * o.dloss_stride];
+    } else {
+      g = pair_slope(pair, o.log_ratio, seq);
+      dl = o.dloss[(seq < pair.pairs ? seq : seq - pair.pairs) * o.dloss_stride];
+    }
+    gt.k1 = -(dl * g) * a.scale_f;
+    grad_row<T, V, 4>(xr, yr, a, gt, logp, col, threadIdx.x, blockDim.x);
+  }
+}
+
+constexpr int kFusedThreads = 1024;
+
+// Loss and gradient in one kernel: a CTA a row; the second reading of the row comes from L2.
+template <typename T, int V>
+__global__ void __launch_bounds__(kFusedThreads, 1) policy_fused_kernel(const LossRows a, const PolicyTerms pol,
+                                                                        const LossOut o, const GradOut go) {
+  __shared__ float red[2][32];
+  const int t = threadIdx.x;
+  uint64_t pol_keep;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol_keep));
+  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
+    const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+    T* yr = static_cast<T*>(go.dx) + r * go.ldo;
+    const int64_t col = label_col(a, r);
+    if (col < 0) {
+      zero_row<T, V>(yr, a, t, kFusedThreads);
+      if (t == 0) o.loss[r] = o.logp[r] = o.lse[r] = o.kl[r] = 0.f;
+      continue;
+    }
+    const float xl = to_f(xr[col]), dl = go.dloss[r * go.dloss_stride];
+    Stat st;
+    fold_row<T, V, 4>(st, xr, a, t, kFusedThreads, [&](const void* p) {
+      Vec16 v;
+      asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+                   : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
+                   : "l"(p), "l"(pol_keep));
+      return v;
+    });
+    const float gm = group_reduce<MaxOp>(st.m, red[0], kFusedThreads / 32, 0);
+    const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], kFusedThreads / 32, 0);
+    const RowStat rs(gm, gs, a);
+    const double logp = rs.logp(a, xl);
+    const PolicyRow p = policy_row(pol, r, logp);
+    if (t == 0) {
+      o.loss[r] = p.loss;
+      o.logp[r] = static_cast<float>(logp);
+      o.lse[r] = static_cast<float>(rs.lse(a));
+      o.kl[r] = p.kl;
+    }
+    // p = 2^((x - m) c - log2 s)
+    const GradTerms gt{-(dl * p.g) * a.scale_f, -rs.m, a.c_hi, -rs.log2s};
+    grad_row<T, V, 2>(xr, yr, a, gt, logp, col, t, kFusedThreads);
+  }
+}
+
+namespace {
+
+template <int KIND, typename T, int V>
+cudaError_t launch_rows(LossRows a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o, cudaStream_t st) {
+  // about 16 vectors (or 64 scalars) a thread, at most 256 threads a row
+  const int64_t units = V > 1 ? (a.nvec + 15) / 16 : (a.N + 63) / 64;
+  a.tpr = static_cast<int>(units >= 256 ? 256 : (units + 31) / 32 * 32);
+  a.rpc = 256 / a.tpr;
+  const int block = a.tpr * a.rpc;
+  const void* fn = reinterpret_cast<const void*>(&loss_rows_kernel<KIND, T, V>);
+  const int grid = persistent_grid(fn, block, 0, (a.M + a.rpc - 1) / a.rpc);
+  loss_rows_kernel<KIND, T, V><<<grid, block, 0, st>>>(a, pol, pair, o);
+  return cudaGetLastError();
+}
+
+template <int KIND, typename T, int V>
+cudaError_t launch_bwd(const LossRows& a, const PolicyTerms& pol, const PairTerms& pair, const GradOut& o,
+                       cudaStream_t st) {
+  const void* fn = reinterpret_cast<const void*>(&loss_bwd_kernel<KIND, T, V>);
+  loss_bwd_kernel<KIND, T, V><<<persistent_grid(fn, 256, 0, a.M), 256, 0, st>>>(a, pol, pair, o);
+  return cudaGetLastError();
+}
+
+template <typename T, int V>
+cudaError_t launch_fused(const LossRows& a, const PolicyTerms& pol, const LossOut& o, const GradOut& go,
+                         cudaStream_t st) {
+  const int64_t cap = sm_count();  // rows in flight stay in L2
+  policy_fused_kernel<T, V><<<static_cast<int>(a.M < cap ? a.M : cap), kFusedThreads, 0, st>>>(a, pol, o, go);
+  return cudaGetLastError();
+}
+
+enum Way { kFwd, kBwd, kFwdBwd };
+
+template <int KIND, typename T, int V>
+cudaError_t launch_way(Way way, LossRows a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o,
+                       const GradOut& go, cudaStream_t st) {
+  a.nvec = V > 1 ? static_cast<int>(a.N / V) : 0;
+  if (way == kFwd) return launch_rows<KIND, T, V>(a, pol, pair, o, st);
+  if (way == kBwd) return launch_bwd<KIND, T, V>(a, pol, pair, go, st);
+  if constexpr (KIND == kPolicy) return launch_fused<T, V>(a, pol, o, go, st);
+  return cudaErrorNotSupported;
+}
+
+template <int KIND, typename T>
+cudaError_t dispatch_vec(Way way, const LossRows& a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o,
+                         const GradOut& go, cudaStream_t st) {
+  constexpr int E = Elt<T>::kPerVec;
+  const bool vec = kernel_path() != DSLPG_PATH_STREAM && aligned(a.x, 16) && a.N % E == 0 && a.ld % E == 0 &&
+                   (way == kFwd || (aligned(go.dx, 16) && go.ldo % E == 0));
+  return vec ? launch_way<KIND, T, E>(way, a, pol, pair, o, go, st) : launch_way<KIND, T, 1>(way, a, pol, pair, o, go, st);
+}
+
+template <int KIND>
+cudaError_t dispatch(Way way, int dt, const LossRows& a, const PolicyTerms& pol, const PairTerms& pair,
+                     const LossOut& o, const GradOut& go, cudaStream_t st) {
+  switch (dt) {
+    case DSLPG_F32: return dispatch_vec<KIND, float>(way, a, pol, pair, o, go, st);
+    case DSLPG_F16: return dispatch_vec<KIND, __half>(way, a, pol, pair, o, go, st);
+    default: return dispatch_vec<KIND, __nv_bfloat16>(way, a, pol, pair, o, go, st);
+  }
+}
+
+bool finite(double v) { return v - v == 0.0; }
+
+int rows_args(LossRows& a, const dslpg_logit_rows* h) {
+  if (!h) return DSLPG_ERR_NULL_POINTER;
+  if (!is_float_dtype(h->logits_dtype) || (h->labels_dtype != DSLPG_I32 && h->labels_dtype != DSLPG_I64))
+    return DSLPG_ERR_BAD_DTYPE;
+  if (h->n_rows < 0 || h->n_cols < 1 || h->n_cols > (1ll << 30) || h->row_stride < h->n_cols) return DSLPG_ERR_BAD_SHAPE;
+  if (!finite(h->logit_scale)) return DSLPG_ERR_BAD_ARGUMENT;
+  if (h->n_rows > 0 && (!h->logits || !h->labels)) return DSLPG_ERR_NULL_POINTER;
+  a.x = h->logits;
+  a.labels = h->labels;
+  a.M = h->n_rows;
+  a.N = h->n_cols;
+  a.ld = h->row_stride;
+  a.ignored = h->ignored_index;
+  a.label64 = h->labels_dtype == DSLPG_I64 ? 1 : 0;
+  a.scale = h->logit_scale;
+  const double c = h->logit_scale * 1.4426950408889634074;  // log2(e)
+  a.scale_f = static_cast<float>(h->logit_scale);
+  a.sign = h->logit_scale < 0 ? -1.f : 1.f;
+  a.c_hi = static_cast<float>(c);
+  if (fabs(static_cast<double>(a.c_hi)) > fabs(c)) a.c_hi = nextafterf(a.c_hi, 0.f);
+  a.c_lo = static_cast<float>(c - static_cast<double>(a.c_hi));
+  if (a.c_lo == 0.f && a.c_hi != 0.f) a.c_lo = copysignf(1.17549435e-38f, a.c_hi);
+  return DSLPG_OK;
+}
+
+int policy_args(PolicyTerms& p, const dslpg_policy_terms* h, int64_t rows) {
+  if (!h) return DSLPG_ERR_NULL_POINTER;
+  if (rows > 0 && (!h->old_logp || !h->advantages)) return DSLPG_ERR_NULL_POINTER;
+  if (h->old_stride < 0 || h->advantages_stride < 0 || h->ref_stride < 0) return DSLPG_ERR_BAD_SHAPE;
+  if (!(h->clip_low >= 0.f && h->clip_low <= 1.f) || !(h->clip_high >= 0.f) || !finite(h->kl_coef))
+    return DSLPG_ERR_BAD_ARGUMENT;
+  p.old_logp = h->old_logp;
+  p.adv = h->advantages;
+  p.ref = h->ref_logp;
+  p.old_stride = h->old_stride;
+  p.adv_stride = h->advantages_stride;
+  p.ref_stride = h->ref_stride;
+  p.lo = 1.f - h->clip_low;
+  p.hi = 1.f + h->clip_high;
+  p.kl_coef = h->kl_coef;
+  return DSLPG_OK;
+}
+
+int pair_args(PairTerms& p, const dslpg_pair_terms* h, int64_t rows, bool fwd) {
+  if (!h) return DSLPG_ERR_NULL_POINTER;
+  if (h->starts_dtype != DSLPG_I32 && h->starts_dtype != DSLPG_I64) return DSLPG_ERR_BAD_DTYPE;
+  if (h->n_pairs < 1 || h->n_pairs > (1ll << 30) || h->ref_stride < 0) return DSLPG_ERR_BAD_SHAPE;
+  if (!h->seq_starts || (fwd && rows > 0 && !h->ref_logp)) return DSLPG_ERR_NULL_POINTER;
+  if (!finite(h->beta) || !(h->smoothing >= 0.f && h->smoothing <= 1.f)) return DSLPG_ERR_BAD_ARGUMENT;
+  p.starts = h->seq_starts;
+  p.starts64 = h->starts_dtype == DSLPG_I64 ? 1 : 0;
+  p.pairs = h->n_pairs;
+  p.ref = h->ref_logp;
+  p.ref_stride = h->ref_stride;
+  p.beta = h->beta;
+  p.smoothing = h->smoothing;
+  return DSLPG_OK;
+}
+
+}  // namespace
+}  // namespace dslpg
+
+using namespace dslpg;
+
+extern "C" int dslpg_policy_loss_fwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms, float* loss,
+                                     float* logp, float* lse, float* kl, cudaStream_t stream) {
+  LossRows a{};
+  PolicyTerms p{};
+  if (int rc = rows_args(a, rows)) return rc;
+  if (int rc = policy_args(p, terms, a.M)) return rc;
+  if (a.M == 0) return DSLPG_OK;
+  if (!loss || !logp || !lse || !kl) return DSLPG_ERR_NULL_POINTER;
+  return static_cast<int>(
+      dispatch<kPolicy>(kFwd, rows->logits_dtype, a, p, PairTerms{}, LossOut{loss, logp, lse, kl}, GradOut{}, stream));
+}
+
+extern "C" int dslpg_policy_loss_bwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms, const float* dloss,
+                                     int64_t dloss_stride, const float* lse, void* dlogits, int64_t dlogits_row_stride,
+                                     cudaStream_t stream) {
+  LossRows a{};
+  PolicyTerms p{};
+  if (int rc = rows_args(a, rows)) return rc;
+  if (int rc = policy_args(p, terms, a.M)) return rc;
+  if (dloss_stride < 0 || dlogits_row_stride < a.N) return DSLPG_ERR_BAD_SHAPE;
+  if (a.M == 0) return DSLPG_OK;
+  if (!dloss || !lse || !dlogits) return DSLPG_ERR_NULL_POINTER;
+  return static_cast<int>(dispatch<kPolicy>(kBwd, rows->logits_dtype, a, p, PairTerms{}, LossOut{},
+                                            GradOut{dloss, dloss_stride, lse, nullptr, dlogits, dlogits_row_stride},
+                                            stream));
+}
+
+extern "C" int dslpg_policy_loss_fwd_bwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms,
+                                         const float* dloss, int64_t dloss_stride, float* loss, float* logp, float* lse,
+                                         float* kl, void* dlogits, int64_t dlogits_row_stride, cudaStream_t stream) {
+  LossRows a{};
+  PolicyTerms p{};
+  if (int rc = rows_args(a, rows)) return rc;
+  if (int rc = policy_args(p, terms, a.M)) return rc;
+  if (dloss_stride < 0 || dlogits_row_stride < a.N) return DSLPG_ERR_BAD_SHAPE;
+  if (a.M == 0) return DSLPG_OK;
+  if (!dloss || !loss || !logp || !lse || !kl || !dlogits) return DSLPG_ERR_NULL_POINTER;
+  return static_cast<int>(dispatch<kPolicy>(kFwdBwd, rows->logits_dtype, a, p, PairTerms{}, LossOut{loss, logp, lse, kl},
+                                            GradOut{dloss, dloss_stride, nullptr, nullptr, dlogits, dlogits_row_stride},
+                                            stream));
+}
+
+extern "C" int dslpg_preference_loss_fwd(const dslpg_logit_rows* rows, const dslpg_pair_terms* terms, float* loss,
+                                         float* log_ratio, float* logp, float* lse, cudaStream_t stream) {
+  LossRows a{};
+  PairTerms p{};
+  if (int rc = rows_args(a, rows)) return rc;
+  if (int rc = pair_args(p, terms, a.M, true)) return rc;
+  if (!loss || !log_ratio || (a.M > 0 && (!logp || !lse))) return DSLPG_ERR_NULL_POINTER;
+  if (a.M > 0) {
+    const cudaError_t e = dispatch<kPair>(kFwd, rows->logits_dtype, a, PolicyTerms{}, p,
+                                          LossOut{nullptr, logp, lse, nullptr}, GradOut{}, stream);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const int grid = static_cast<int>(p.pairs < 65535 ? p.pairs : 65535);
+  pair_kernel<<<grid, 256, 0, stream>>>(a, p, logp, loss, log_ratio);
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int dslpg_preference_loss_bwd(const dslpg_logit_rows* rows, const dslpg_pair_terms* terms,
+                                         const float* dloss, int64_t dloss_stride, const float* lse,
+                                         const float* log_ratio, void* dlogits, int64_t dlogits_row_stride,
+                                         cudaStream_t stream) {
+  LossRows a{};
+  PairTerms p{};
+  if (int rc = rows_args(a, rows)) return rc;
+  if (int rc = pair_args(p, terms, a.M, false)) return rc;
+  if (dloss_stride < 0 || dlogits_row_stride < a.N) return DSLPG_ERR_BAD_SHAPE;
+  if (a.M == 0) return DSLPG_OK;
+  if (!dloss || !lse || !log_ratio || !dlogits) return DSLPG_ERR_NULL_POINTER;
+  return static_cast<int>(dispatch<kPair>(kBwd, rows->logits_dtype, a, PolicyTerms{}, p, LossOut{},
+                                          GradOut{dloss, dloss_stride, lse, log_ratio, dlogits, dlogits_row_stride},
+                                          stream));
+}

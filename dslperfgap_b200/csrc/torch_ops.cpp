@@ -424,6 +424,175 @@ py::object qk_norm_rope_bwd(py::handle dq_, py::handle dk_, py::handle q, py::ha
   return py::make_tuple(dq, dk, dqw, dkw);
 }
 
+// A float32 CUDA vector of n values on `dev`.
+std::optional<at::Tensor> f32_vector(const py::handle& h, int dev, int64_t n, bool dense = false) {
+  auto t = cuda_of(h, dev, at::kFloat, at::kFloat);
+  if (!t || t->dim() != 1 || t->size(0) != n || (dense && !t->is_contiguous())) return std::nullopt;
+  return t;
+}
+
+// Logits and labels of the losses (policy_loss, preference_loss).
+struct LossRows {
+  at::Tensor logits, labels;
+  dslpg_logit_rows r{};
+
+  bool take(py::handle x_, py::handle labels_, py::handle scale, py::handle ignored) {
+    auto x = cuda_float(x_);
+    if (!x || x->dim() != 2 || x->size(0) == 0 || x->size(1) < 1 || x->size(1) > (1ll << 30) || x->stride(1) != 1 ||
+        (x->size(0) > 1 && x->stride(0) < x->size(1)) || !is_number(scale) || !is_int(ignored))
+      return false;
+    auto lab = cuda_of(labels_, x->get_device(), at::kLong, at::kInt);
+    if (!lab || lab->dim() != 1 || lab->size(0) != x->size(0) || !lab->is_contiguous()) return false;
+    logits = *x;
+    labels = *lab;
+    r.logits = logits.data_ptr();
+    r.labels = labels.data_ptr();
+    r.n_rows = x->size(0);
+    r.n_cols = x->size(1);
+    r.row_stride = x->size(0) > 1 ? x->stride(0) : x->size(1);
+    r.ignored_index = ignored.cast<int64_t>();
+    r.logit_scale = scale.cast<double>();
+    r.logits_dtype = float_code(x->scalar_type());
+    r.labels_dtype = lab->scalar_type() == at::kLong ? DSLPG_I64 : DSLPG_I32;
+    return r.logit_scale - r.logit_scale == 0.0;
+  }
+  int dev() const { return logits.get_device(); }
+  at::Tensor f32(int64_t n) const { return at::empty({n}, logits.options().dtype(at::kFloat)); }
+  at::Tensor grad() const { return at::empty(logits.sizes(), logits.options()); }
+};
+
+struct Policy {
+  at::Tensor old, adv, ref;
+  dslpg_policy_terms t{};
+
+  bool take(const LossRows& r, py::handle old_, py::handle adv_, py::handle ref_, py::handle low, py::handle high,
+            py::handle kl) {
+    auto o = f32_vector(old_, r.dev(), r.r.n_rows), a = f32_vector(adv_, r.dev(), r.r.n_rows);
+    if (!o || !a || !is_number(low) || !is_number(high) || !is_number(kl)) return false;
+    if (!ref_.is_none()) {
+      auto f = f32_vector(ref_, r.dev(), r.r.n_rows);
+      if (!f) return false;
+      ref = *f;
+      t.ref_logp = ref.data_ptr<float>();
+      t.ref_stride = ref.stride(0);
+    }
+    old = *o;
+    adv = *a;
+    t.old_logp = old.data_ptr<float>();
+    t.advantages = adv.data_ptr<float>();
+    t.old_stride = old.stride(0);
+    t.advantages_stride = adv.stride(0);
+    const double lo = low.cast<double>(), hi = high.cast<double>(), k = kl.cast<double>();
+    t.clip_low = static_cast<float>(lo);
+    t.clip_high = static_cast<float>(hi);
+    t.kl_coef = static_cast<float>(k);
+    return lo >= 0 && lo <= 1 && hi >= 0 && t.kl_coef - t.kl_coef == 0.f;
+  }
+};
+
+py::object policy_loss_fwd(py::handle x, py::handle labels, py::handle old, py::handle adv, py::handle ref,
+                           py::handle low, py::handle high, py::handle kl_coef, py::handle scale, py::handle ignored) {
+  LossRows r;
+  Policy p;
+  if (!r.take(x, labels, scale, ignored) || !p.take(r, old, adv, ref, low, high, kl_coef)) return py::none();
+  const int64_t n = r.r.n_rows;
+  at::Tensor loss = r.f32(n), logp = r.f32(n), lse = r.f32(n), kl = r.f32(n);
+  launch(r.logits, "dslpg_policy_loss_fwd", [&](cudaStream_t s) {
+    return dslpg_policy_loss_fwd(&r.r, &p.t, loss.data_ptr<float>(), logp.data_ptr<float>(), lse.data_ptr<float>(),
+                                 kl.data_ptr<float>(), s);
+  });
+  return py::make_tuple(loss, logp, lse, kl);
+}
+
+py::object policy_loss_bwd(py::handle dloss_, py::handle x, py::handle lse_, py::handle labels, py::handle old,
+                           py::handle adv, py::handle ref, py::handle low, py::handle high, py::handle kl_coef,
+                           py::handle scale, py::handle ignored) {
+  LossRows r;
+  Policy p;
+  if (!r.take(x, labels, scale, ignored) || !p.take(r, old, adv, ref, low, high, kl_coef)) return py::none();
+  auto dloss = f32_vector(dloss_, r.dev(), r.r.n_rows), lse = f32_vector(lse_, r.dev(), r.r.n_rows, true);
+  if (!dloss || !lse) return py::none();
+  at::Tensor dx = r.grad();
+  launch(r.logits, "dslpg_policy_loss_bwd", [&](cudaStream_t s) {
+    return dslpg_policy_loss_bwd(&r.r, &p.t, dloss->data_ptr<float>(), dloss->stride(0), lse->data_ptr<float>(),
+                                 dx.data_ptr(), r.r.n_cols, s);
+  });
+  return py::cast(dx);
+}
+
+py::object policy_loss_fwd_bwd(py::handle x, py::handle labels, py::handle old, py::handle adv, py::handle dloss_,
+                               py::handle ref, py::handle low, py::handle high, py::handle kl_coef, py::handle scale,
+                               py::handle ignored) {
+  LossRows r;
+  Policy p;
+  if (!r.take(x, labels, scale, ignored) || !p.take(r, old, adv, ref, low, high, kl_coef)) return py::none();
+  const int64_t n = r.r.n_rows;
+  auto dloss = f32_vector(dloss_, r.dev(), n);
+  if (!dloss) return py::none();
+  at::Tensor loss = r.f32(n), logp = r.f32(n), lse = r.f32(n), kl = r.f32(n), dx = r.grad();
+  launch(r.logits, "dslpg_policy_loss_fwd_bwd", [&](cudaStream_t s) {
+    return dslpg_policy_loss_fwd_bwd(&r.r, &p.t, dloss->data_ptr<float>(), dloss->stride(0), loss.data_ptr<float>(),
+                                     logp.data_ptr<float>(), lse.data_ptr<float>(), kl.data_ptr<float>(),
+                                     dx.data_ptr(), r.r.n_cols, s);
+  });
+  return py::make_tuple(loss, logp, lse, kl, dx);
+}
+
+struct Pairs {
+  at::Tensor starts;
+  dslpg_pair_terms t{};
+
+  bool take(const LossRows& r, py::handle starts_, py::handle beta, py::handle smoothing) {
+    auto st = cuda_of(starts_, r.dev(), at::kLong, at::kInt);
+    if (!st || st->dim() != 1 || st->size(0) < 3 || st->size(0) % 2 == 0 || !st->is_contiguous() ||
+        !is_number(beta) || !is_number(smoothing))
+      return false;
+    starts = *st;
+    t.seq_starts = starts.data_ptr();
+    t.starts_dtype = starts.scalar_type() == at::kLong ? DSLPG_I64 : DSLPG_I32;
+    t.n_pairs = starts.size(0) / 2;
+    const double s = smoothing.cast<double>();
+    t.beta = static_cast<float>(beta.cast<double>());
+    t.smoothing = static_cast<float>(s);
+    return s >= 0 && s <= 1 && t.beta - t.beta == 0.f;
+  }
+};
+
+py::object preference_loss_fwd(py::handle x, py::handle labels, py::handle starts, py::handle ref_, py::handle beta,
+                               py::handle smoothing, py::handle scale, py::handle ignored) {
+  LossRows r;
+  Pairs p;
+  if (!r.take(x, labels, scale, ignored) || !p.take(r, starts, beta, smoothing)) return py::none();
+  auto ref = f32_vector(ref_, r.dev(), r.r.n_rows);
+  if (!ref) return py::none();
+  p.t.ref_logp = ref->data_ptr<float>();
+  p.t.ref_stride = ref->stride(0);
+  at::Tensor loss = r.f32(p.t.n_pairs), ratio = r.f32(2 * p.t.n_pairs), logp = r.f32(r.r.n_rows),
+             lse = r.f32(r.r.n_rows);
+  launch(r.logits, "dslpg_preference_loss_fwd", [&](cudaStream_t s) {
+    return dslpg_preference_loss_fwd(&r.r, &p.t, loss.data_ptr<float>(), ratio.data_ptr<float>(),
+                                     logp.data_ptr<float>(), lse.data_ptr<float>(), s);
+  });
+  return py::make_tuple(loss, ratio, logp, lse);
+}
+
+py::object preference_loss_bwd(py::handle dloss_, py::handle x, py::handle lse_, py::handle labels, py::handle starts,
+                               py::handle ratio_, py::handle beta, py::handle smoothing, py::handle scale,
+                               py::handle ignored) {
+  LossRows r;
+  Pairs p;
+  if (!r.take(x, labels, scale, ignored) || !p.take(r, starts, beta, smoothing)) return py::none();
+  auto dloss = f32_vector(dloss_, r.dev(), p.t.n_pairs), lse = f32_vector(lse_, r.dev(), r.r.n_rows, true),
+       ratio = f32_vector(ratio_, r.dev(), 2 * p.t.n_pairs, true);
+  if (!dloss || !lse || !ratio) return py::none();
+  at::Tensor dx = r.grad();
+  launch(r.logits, "dslpg_preference_loss_bwd", [&](cudaStream_t s) {
+    return dslpg_preference_loss_bwd(&r.r, &p.t, dloss->data_ptr<float>(), dloss->stride(0), lse->data_ptr<float>(),
+                                     ratio->data_ptr<float>(), dx.data_ptr(), r.r.n_cols, s);
+  });
+  return py::cast(dx);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dslpg_torch, m) {
@@ -437,6 +606,11 @@ PYBIND11_MODULE(_dslpg_torch, m) {
   m.def("max_reduction", &max_reduction);
   m.def("argmax", &argmax);
   m.def("cross_entropy_fwd", &cross_entropy_fwd);
+  m.def("policy_loss_fwd", &policy_loss_fwd);
+  m.def("policy_loss_bwd", &policy_loss_bwd);
+  m.def("policy_loss_fwd_bwd", &policy_loss_fwd_bwd);
+  m.def("preference_loss_fwd", &preference_loss_fwd);
+  m.def("preference_loss_bwd", &preference_loss_bwd);
   m.def("rope", &rope);
   m.def("rope_bwd", &rope_bwd);
   m.def("qk_norm_rope", &qk_norm_rope);

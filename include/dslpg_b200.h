@@ -360,6 +360,84 @@ DSLPG_API int dslpg_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, con
                                      const dslpg_heads* heads, float eps, void* workspace, int64_t workspace_bytes,
                                      cudaStream_t stream);
 
+/*
+ * Losses of post-training on rows of logits, with their gradients: the clipped
+ * policy loss with a KL term, and the preference loss on paired sequences.
+ *
+ * logits [n_rows, n_cols] of logits_dtype, rows row_stride elements apart;
+ * labels [n_rows] (int32 or int64), dense. With z = logit_scale * logits:
+ * lse = log sum exp z, logp = z[label] - lse (both float32 outputs [n_rows]).
+ * A row whose label is ignored_index, or no column, is left out: its logits are
+ * not read, and its loss, logp, lse, kl and gradient are 0. n_cols <= 2^30.
+ * No reference counterpart: the suite has the cross-entropy of such rows.
+ */
+typedef struct dslpg_logit_rows {
+  const void* logits;
+  const void* labels;
+  int64_t n_rows, n_cols, row_stride, ignored_index;
+  double logit_scale;
+  int32_t logits_dtype, labels_dtype;
+} dslpg_logit_rows;
+
+/*
+ * Per row, with old = old_logp, A = advantages, ref = ref_logp (float32, each
+ * with its own stride; 0: one value for all rows):
+ *   r = exp(logp - old);  d = ref - logp;  kl = exp(d) - d - 1  (0 when ref_logp is NULL)
+ *   loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl
+ *   g = dloss/dlogp = (0 where the clipped term alone counts, else -r A) + kl_coef (1 - exp(d))
+ *   dlogits = dloss g logit_scale (onehot(label) - softmax(z))
+ * 0 <= clip_low <= 1, clip_high >= 0. With kl_coef 0 the KL term is only reported.
+ */
+typedef struct dslpg_policy_terms {
+  const float* old_logp;
+  const float* advantages;
+  const float* ref_logp;
+  int64_t old_stride, advantages_stride, ref_stride;
+  float clip_low, clip_high, kl_coef;
+  float reserved;
+} dslpg_policy_terms;
+
+DSLPG_API int dslpg_policy_loss_fwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms, float* loss,
+                                    float* logp, float* lse, float* kl, cudaStream_t stream);
+
+/* dlogits (logits_dtype, rows dlogits_row_stride apart) from the forward's lse
+ * and the losses' gradients dloss (float32 [n_rows], stride dloss_stride). */
+DSLPG_API int dslpg_policy_loss_bwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms, const float* dloss,
+                                    int64_t dloss_stride, const float* lse, void* dlogits, int64_t dlogits_row_stride,
+                                    cudaStream_t stream);
+
+/* Both in one pass over the logits, for a dloss known beforehand. */
+DSLPG_API int dslpg_policy_loss_fwd_bwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms,
+                                        const float* dloss, int64_t dloss_stride, float* loss, float* logp, float* lse,
+                                        float* kl, void* dlogits, int64_t dlogits_row_stride, cudaStream_t stream);
+
+/*
+ * 2 n_pairs sequences of rows: sequence s is rows seq_starts[s] to
+ * seq_starts[s + 1] (2 n_pairs + 1 ascending bounds, int32 or int64); the
+ * chosen ones come first, pair k is sequences k and n_pairs + k. Rows before
+ * the first bound or from the last one on are left out.
+ *   log_ratio[s] = sum of logp - ref_logp over the rows of s that are not left out
+ *   m = beta (log_ratio[k] - log_ratio[n_pairs + k])
+ *   loss[k] = (1 - smoothing) softplus(-m) + smoothing softplus(m)
+ * The sums are held in 64 bits, in a fixed order. 0 <= smoothing <= 1.
+ */
+typedef struct dslpg_pair_terms {
+  const void* seq_starts;
+  const float* ref_logp; /* not read by the backward */
+  int64_t n_pairs, ref_stride;
+  float beta, smoothing;
+  int32_t starts_dtype, reserved;
+} dslpg_pair_terms;
+
+DSLPG_API int dslpg_preference_loss_fwd(const dslpg_logit_rows* rows, const dslpg_pair_terms* terms, float* loss,
+                                        float* log_ratio, float* logp, float* lse, cudaStream_t stream);
+
+/* dlogits from the forward's lse and log_ratio and the pairs' dloss (float32 [n_pairs]). */
+DSLPG_API int dslpg_preference_loss_bwd(const dslpg_logit_rows* rows, const dslpg_pair_terms* terms,
+                                        const float* dloss, int64_t dloss_stride, const float* lse,
+                                        const float* log_ratio, void* dlogits, int64_t dlogits_row_stride,
+                                        cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
