@@ -128,7 +128,8 @@ extern "C" int dslpg_set_kernel_path(int path) {
 extern "C" int dslpg_get_kernel_path(void) { return dslpg::g_path; }
 
 extern "C" unsigned int dslpg_take_wait_timeouts(void) {
-  return dslpg::take_wait_timeouts_rownorm() + dslpg::take_wait_timeouts_rowstat() + dslpg::take_wait_timeouts_ff();
+  return dslpg::take_wait_timeouts_rownorm() + dslpg::take_wait_timeouts_rowstat() + dslpg::take_wait_timeouts_ff() +
+         dslpg::take_wait_timeouts_heads();
 }
 
 extern "C" int dslpg_version(void) { return (0 << 16) | 1; }

@@ -430,6 +430,7 @@ int kernel_path();
 unsigned int take_wait_timeouts_rownorm();
 unsigned int take_wait_timeouts_rowstat();
 unsigned int take_wait_timeouts_ff();
+unsigned int take_wait_timeouts_heads();
 
 inline int dtype_size(int dt) { return dt == DSLPG_F32 ? 4 : 2; }
 inline bool is_float_dtype(int dt) { return dt == DSLPG_F32 || dt == DSLPG_F16 || dt == DSLPG_BF16; }

@@ -10,22 +10,37 @@
 //   dx = rstd * (w g - x rstd^2 c / D);  dw = sum over rows of g x rstd.
 // The rotation's own backward is the rotation by -phi.
 //
-// Angles: pos * f_i is formed in 64 bits as turns, pos * (f_i / 2 pi), its
-// whole turns are dropped exactly, and the fraction goes to sincospi in 32
-// bits; far positions (1e6 and more) keep the cosine to 32-bit accuracy. The
-// n angles of a token serve all of its heads, so one warp takes a token (or
-// part of its heads when there are few tokens), computes the angles once into
-// its own slice of shared memory and then walks the heads.
+// Angles: as fractions of a turn in 64-bit fixed point, where f_i / 2 pi times an
+// integer position is one wrapping integer product: the whole turns fall off
+// exactly, for negative and far positions (1e6 and more) alike, and the cosine
+// keeps its 32-bit accuracy. (The same in double precision took 0.9 us a token
+// in its warp, a chain of conversions and roundings.) The n angles of a token
+// are formed once and serve all of its heads.
 //
 // Lanes: a row is cut into units of two V-element vectors that hold both
 // members of V rotated pairs (vectors u and u + n/V; interleaved 2u and
 // 2u + 1), so the rotation needs no exchange between lanes; the features
-// past R are units of two neighbouring vectors. L lanes (a power of two) hold
-// a row, 32 / L rows go through a warp at a time.
+// past R are units of two neighbouring vectors. A lane takes one unit, a warp
+// takes 32 / units rows (a group) at a time.
+//
+// Pipeline: a CTA walks tiles of a few whole tokens (or of some heads of one).
+// Warp 0 copies a tile's rows into a ring of shared-memory stages with
+// cp.async.bulk, the next warps form its tokens' angles there, and the other
+// warps turn rows into outputs. Rows lie in a stage as in the output, tensor by
+// tensor, so a row's place in both is its number, and a group may span tokens.
+// Before this, each warp copied its own rows (cp.async, one lane a vector) and
+// formed its own angles; the addresses, bounds and waits of that took 200 of 440
+// instructions a group of rows: forward 61.0 us against
+// 59.5 for 16384 tokens of 32 + 8 heads of 128 in bf16 (the same bytes copied by
+// cudaMemcpy's kernel: 58), the rotation of 29971 tokens of 16 + 16 heads 86.8
+// against 86.0 (81.5), and one decoded token 6.2 against 4.2.
 #include "common.cuh"
 #include "pipe.cuh"
 
 namespace dslpg {
+
+// Waits that ran out of time in this file's kernels.
+static __device__ unsigned int g_heads_timeouts;
 
 struct HeadArgs {
   const void* x[2];    // q, k: the rows (rotation backward: dy)
@@ -34,7 +49,7 @@ struct HeadArgs {
   const void* w[2];    // [D] weights
   const void* pos;
   const float* inv_freq;
-  float* partial;      // norm backward: [CTAs][D] sums for dw
+  float* partial;      // norm backward: [CTAs][2][D] sums for dw
   int64_t xs[2][3];    // batch, sequence and head strides of x
   int64_t dys[2][3];
   int64_t ps[3];       // axis, batch and sequence strides of pos
@@ -42,295 +57,611 @@ struct HeadArgs {
   int heads[2];
   int D, n;            // features; rotated pairs
   int bound[3];        // first frequency of axes 1, 2, 3
-  int rot_units, units, log_l;
-  int groups[2];       // groups of 32 / L heads
-  uint32_t chunk, chunks;  // groups per item, items per token (norm backward: of q's CTAs)
-  uint32_t chunk_k, chunks_k;  // norm backward: of k's CTAs
-  int q_ctas;          // norm backward: the first q_ctas CTAs take q, the others k
+  int axes;
+  int rot_units, units, rpw;  // rpw: rows of a group, 32 / units
+  // Tiles: tt tokens with all their heads, or (parts > 1) one token and `part` of its heads.
+  int tt, part, parts;
+  uint32_t tiles;
+  int stages, stage_bytes, row_bytes;
+  int angle_warps, row_warps;
+  int groups;          // groups of a tile: those of q's rows, then those of k's (the last ones may be empty)
+  // From a tile of a CTA to its next one (parts == 1): tokens modulo seq; what is
+  // added to a token's place in x, dy and pos, and once more where a sequence ends.
+  uint32_t s_step;
+  int64_t x_step[2], x_carry[2], dy_step[2], dy_carry[2], p_step, p_carry;
+  uint32_t magic[2];   // r / heads of a token in the tile = umulhi(r, magic); 0: r itself
   int wdt, pos64, interleaved;
   float eps, inv_d, sign;
 };
 
-// V elements of T in 32-bit words.
+enum HeadOp : int { kRotate, kNorm, kNormBwd };
+
+// V elements of T.
 template <typename T, int V> struct Pack {
-  static constexpr int kWords = V * static_cast<int>(sizeof(T)) / 4;
-  uint32_t w[kWords];
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  static_assert(kBytes == 8 || kBytes == 16, "8- or 16-byte vectors");
 };
 
-template <typename T, int V> DSLPG_DEV void ld_pack(Pack<T, V>& p, const T* src) {
-  if constexpr (Pack<T, V>::kWords == 4) {
-    const Vec16 v = ld_stream(src);
+// Plain float32 arithmetic throughout: packed pairs (fma.f32x2) took more
+// instructions here (48 M against 41 M for a rotation of 29971 tokens of 32
+// heads), as their operands have to be moved into register pairs.
+template <typename T, int V> DSLPG_DEV void lds_vec(uint32_t at, float (&f)[V]) {
+  Vec16 v{{0u, 0u, 0u, 0u}};
+  if constexpr (Pack<T, V>::kBytes == 16) v = lds16(at);
+  else asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.w[0]), "=r"(v.w[1]) : "r"(at) : "memory");
+  float all[Elt<T>::kPerVec];
+  unpack<T>(v, all);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p.w[i] = v.w[i];
+  for (int i = 0; i < V; ++i) f[i] = all[i];
+}
+
+template <typename T, int V> DSLPG_DEV void st_vec(T* dst, const float (&f)[V]) {
+  if constexpr (sizeof(T) == 4 && V == 2) st_stream8(dst, __float_as_uint(f[0]), __float_as_uint(f[1]));
+  else StoreOut<T, V>::run(dst, f);
+}
+
+// The part of a turn that one position step makes, in units of 2^-64 turns.
+DSLPG_DEV uint64_t turn_per_step(float f) {
+  const double turns = static_cast<double>(f) * 0.15915494309189533577;  // 1 / (2 pi)
+  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+}
+
+// Cosine and sine (times `sign`) of position p at a frequency's turn_per_step.
+// For 16-bit rows the SFU's, off by at most 2^-20.9 on this range, far inside
+// the rows' own rounding (2^-12, 2^-9) and a fifth of the instructions.
+template <bool EXACT> DSLPG_DEV float2 angle_of(int64_t p, uint64_t step, float sign) {
+  const int turn = static_cast<int>((static_cast<uint64_t>(p) * step) >> 32);  // 2^-32 turns, -2^31 .. 2^31
+  float sn, cn;
+  if constexpr (EXACT) {
+    sincospif(static_cast<float>(turn) * 0x1p-31f, &sn, &cn);
   } else {
-    static_assert(Pack<T, V>::kWords == 2, "8- or 16-byte vectors");
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(p.w[0]), "=r"(p.w[1]) : "l"(src));
+    const float a = static_cast<float>(turn) * 1.4629180793e-9f;  // 2 pi / 2^32
+    sn = __sinf(a);
+    cn = __cosf(a);
   }
+  return make_float2(cn, sn * sign);
 }
 
-template <typename T, int V> DSLPG_DEV void st_pack(T* dst, const float (&f)[V]) {
-  uint32_t w[Pack<T, V>::kWords];
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = __float_as_uint(f[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
-  }
-  if constexpr (Pack<T, V>::kWords == 4) st_stream(dst, Vec16{{w[0], w[1], w[2], w[3]}});
-  else st_stream8(dst, w[0], w[1]);
+DSLPG_DEV int axis_of(const HeadArgs& a, int i) {
+  return i >= a.n ? 0 : (i >= a.bound[0]) + (i >= a.bound[1]) + (i >= a.bound[2]);
 }
 
-template <typename T, int V> DSLPG_DEV void unpack_to(const Pack<T, V>& p, float (&f)[V]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = __uint_as_float(p.w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) upk2(unpack_pair<T>(Vec16{{p.w[i], 0u, 0u, 0u}}, 0), f[2 * i], f[2 * i + 1]);
-  }
+// The positions of the token at `at` in pos: each of the first lanes reads one axis'.
+DSLPG_DEV int64_t lane_position(const HeadArgs& a, int64_t at, int lane) {
+  if (lane >= a.axes) return 0;
+  const int64_t j = at + lane * a.ps[0];
+  return a.pos64 ? static_cast<const int64_t*>(a.pos)[j] : static_cast<const int32_t*>(a.pos)[j];
 }
 
-// Cosines and sines of token (b, s) for this warp: cs[i] = (cos, sin) of frequency i.
-DSLPG_DEV void fill_angles(const HeadArgs& a, float2* cs, uint32_t b, uint32_t s, int lane) {
-  const int64_t at = b * a.ps[1] + s * a.ps[2];
-  for (int i = lane; i < a.n; i += 32) {
-    const int axis = (i >= a.bound[0]) + (i >= a.bound[1]) + (i >= a.bound[2]);
-    const int64_t j = at + axis * a.ps[0];
-    const double p = a.pos64 ? static_cast<double>(static_cast<const int64_t*>(a.pos)[j])
-                             : static_cast<double>(static_cast<const int32_t*>(a.pos)[j]);
-    const double turns = p * (static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577);  // 1 / (2 pi)
-    float sn, cn;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cn);
-    cs[i] = make_float2(cn, sn * a.sign);
+// Angles of a token for this warp, cs[i] = (cos, sin) of frequency i, from its lanes' positions.
+template <bool EXACT> DSLPG_DEV void fill_angles(const HeadArgs& a, const uint64_t* freq, float2* cs, int64_t p, int lane) {
+  __syncwarp();
+  for (int i0 = 0; i0 < a.n; i0 += 32) {
+    const int i = i0 + lane;
+    const int64_t mine = __shfl_sync(0xffffffffu, static_cast<long long>(p), axis_of(a, i));
+    if (i < a.n) cs[i] = angle_of<EXACT>(mine, freq[i], a.sign);
   }
+  __syncwarp();
 }
 
-// Vector indexes of unit u's two vectors; ib < 0: the unit has one vector only.
-template <int V, bool INTER>
+// Vector indexes of unit u's two vectors.
+template <bool INTER>
 DSLPG_DEV void unit_vectors(const HeadArgs& a, int u, int& ia, int& ib) {
-  if (u < a.rot_units) {
-    ia = INTER ? 2 * u : u;
-    ib = INTER ? 2 * u + 1 : u + a.rot_units;
+  const bool half = u < a.rot_units && !INTER;
+  ia = half ? u : 2 * u;  // past the rotated ones: 2 rot_units + 2 (u - rot_units)
+  ib = half ? u + a.rot_units : 2 * u + 1;
+}
+
+// Sums over the `units` lanes of a row, in all of them.
+template <int K> DSLPG_DEV void row_sums(float (&v)[K], int units, int u, int lane) {
+  auto swap = [&](int o) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  };
+  if (units == 8) {  // 128 features of 16 bits, 64 of 32 bits
+    swap(1);
+    swap(2);
+    swap(4);
+  } else if ((units & (units - 1)) == 0) {
+    for (int o = 1; o < units; o <<= 1) swap(o);
   } else {
-    ia = 2 * u;  // 2 rot_units + 2 (u - rot_units)
-    ib = ia + 1 < a.D / V ? ia + 1 : -1;
+    for (int o = 1; o < units; o <<= 1) {  // lane u holds the sum of u .. u + 2 o - 1 inside the row
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float t = __shfl_down_sync(0xffffffffu, v[k], o);
+        if (u + o < units) v[k] += t;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, v[k], lane - u);
   }
 }
 
-// Rotate a unit's pairs in place by the angles c[e] = (cos, sin).
+// What a lane does in the tile kernel.
+template <bool INTER> struct Lane {
+  int u, sub, ia, ib;
+  bool active;
+  DSLPG_DEV Lane(const HeadArgs& a, int lane) {
+    sub = lane / a.units;
+    u = lane - sub * a.units;
+    active = sub < a.rpw;
+    unit_vectors<INTER>(a, u, ia, ib);
+  }
+};
+
+// Tables that a lane reads as its unit's values, four at a time: planes of
+// float4, plane j holding values 4j .. 4j + 3 of every unit (or vector), so that
+// neighbouring lanes read neighbouring 16 bytes.
+//   angles: (cos, sin) of two frequencies in a plane entry, V / 2 planes;
+//   weights: V / 4 planes (one of float2 when V is 2).
+template <int V> DSLPG_DEV int angle_slot(int i, int rot_units) {  // float2 index of frequency i
+  const int u = i / V, e = i - u * V;
+  return ((e >> 1) * rot_units + u) * 2 + (e & 1);
+}
+template <int V> DSLPG_DEV int weight_slot(int d, int vecs) {  // float index of feature d
+  constexpr int P = V < 4 ? V : 4;
+  const int v = d / V, e = d - v * V;
+  return ((e / P) * vecs + v) * P + e % P;
+}
+
+template <int V> DSLPG_DEV void read_weights(const float* w, int vec, int vecs, float (&f)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 q = reinterpret_cast<const float4*>(w)[j * vecs + vec];
+      f[4 * j] = q.x;
+      f[4 * j + 1] = q.y;
+      f[4 * j + 2] = q.z;
+      f[4 * j + 3] = q.w;
+    }
+  } else {
+    const float2 q = reinterpret_cast<const float2*>(w)[vec];
+    f[0] = q.x;
+    f[1] = q.y;
+  }
+}
+
+// Rotate a unit's V pairs in place: half-split (x0 in fa, x1 in fb), or
+// interleaved (2e, 2e + 1 of fa, then of fb).
 template <int V, bool INTER>
-DSLPG_DEV void rotate_unit(float (&fa)[V], float (&fb)[V], const float2 (&c)[V], float sgn) {
-  if constexpr (INTER) {
+DSLPG_DEV void turn(float (&fa)[V], float (&fb)[V], const float4* angles, int rot_units) {
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
-      const float2 p = c[e], q = c[V / 2 + e];
-      const float a0 = fa[2 * e], a1 = fa[2 * e + 1], b0 = fb[2 * e], b1 = fb[2 * e + 1];
-      fa[2 * e] = a0 * p.x - a1 * (p.y * sgn);
-      fa[2 * e + 1] = a1 * p.x + a0 * (p.y * sgn);
-      fb[2 * e] = b0 * q.x - b1 * (q.y * sgn);
-      fb[2 * e + 1] = b1 * q.x + b0 * (q.y * sgn);
-    }
-  } else {
+  for (int j = 0; j < V / 2; ++j) {
+    const float4 cs = angles[j * rot_units];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float x0 = fa[e], x1 = fb[e];
-      fa[e] = x0 * c[e].x - x1 * (c[e].y * sgn);
-      fb[e] = x1 * c[e].x + x0 * (c[e].y * sgn);
+    for (int k = 0; k < 2; ++k) {
+      const int e = 2 * j + k;
+      float& x0 = INTER ? (e < V / 2 ? fa[(2 * e) % V] : fb[(2 * e) % V]) : fa[e];
+      float& x1 = INTER ? (e < V / 2 ? fa[(2 * e) % V + 1] : fb[(2 * e) % V + 1]) : fb[e];
+      const float c = k ? cs.z : cs.x, s = k ? cs.w : cs.y;
+      const float y0 = x0 * c - x1 * s;
+      x1 = x1 * c + x0 * s;
+      x0 = y0;
     }
   }
 }
 
-DSLPG_DEV float lanes_sum(float v, int log_l) {
-  for (int k = 0; k < log_l; ++k) v += __shfl_xor_sync(0xffffffffu, v, 1 << k);
-  return v;
+// Parts of a CTA's dynamic shared memory, in this order.
+struct HeadSmem {
+  int stages, stage_bytes, angle_bytes, n, weight_floats, other_bytes;
+  __host__ __device__ int angles() const { return stages * stage_bytes; }            // [stages][tt][planes]
+  __host__ __device__ int freq() const { return angles() + stages * angle_bytes; }   // uint64 [n]
+  __host__ __device__ int weight() const { return (freq() + 8 * n + 15) & ~15; }     // [2][weight_floats]
+  __host__ __device__ int other() const { return weight() + 8 * weight_floats; }     // [row threads][2 V] floats
+  __host__ __device__ int bars() const { return other() + other_bytes; }
+  __host__ __device__ int total() const { return bars() + 16 * stages; }
+};
+
+__host__ __device__ inline HeadSmem head_smem(const HeadArgs& a, int op, int V) {
+  return HeadSmem{a.stages, a.stage_bytes, (a.tt * a.n * 8 + 15) & ~15, a.n, op == kRotate ? 0 : (a.D + 3) & ~3,
+                  op == kNormBwd ? a.row_warps * 32 * 2 * V * 4 : 0};
 }
 
-template <typename T, int V, bool INTER, bool NORM>
-__global__ void __launch_bounds__(256) heads_fwd_kernel(const HeadArgs a) {
-  extern __shared__ __align__(16) float smem_f[];
-  float* weights = smem_f;  // [2][D] (NORM)
-  float2* table = reinterpret_cast<float2*>(smem_f + (NORM ? 2 * ((a.D + 3) & ~3) : 0));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  float2* cs = table + static_cast<size_t>(warp) * a.n;
-  const int wstride = (a.D + 3) & ~3;
-  if constexpr (NORM) {
+// A tile: tokens [token, token + count), heads [lo, lo + n) of either tensor.
+struct Tile {
+  uint32_t token;
+  int count, lo[2], n[2], rows[2];
+  DSLPG_DEV Tile(const HeadArgs& a, uint32_t tile) {
+    if (a.parts == 1) {
+      token = tile * a.tt;
+      count = min(a.tt, static_cast<int>(a.tokens - token));
+      lo[0] = lo[1] = 0;
+      n[0] = a.heads[0];
+      n[1] = a.heads[1];
+    } else {
+      token = tile / a.parts;
+      count = 1;
+      const int first = static_cast<int>(tile - token * a.parts) * a.part, last = first + a.part;
+      lo[0] = min(first, a.heads[0]);
+      n[0] = min(last, a.heads[0]) - lo[0];
+      lo[1] = max(first - a.heads[0], 0);
+      n[1] = min(max(last - a.heads[0], 0), a.heads[1]) - lo[1];
+    }
+    rows[0] = count * n[0];
+    rows[1] = count * n[1];
+  }
+};
+
+constexpr int kMaxTileTokens = 8;
+
+// Where the k-th token of a CTA's tiles lies in a tensor with batch and sequence
+// strides: divisions at the first tile only (at each with parts > 1).
+struct Place {
+  uint32_t s;
+  int64_t at;
+  DSLPG_DEV void seek(const HeadArgs& a, uint32_t token, int64_t batch, int64_t seq) {
+    const uint32_t b = token / a.seq;
+    s = token - b * a.seq;
+    at = b * batch + s * seq;
+  }
+  DSLPG_DEV void next(const HeadArgs& a, int64_t step, int64_t carry) {
+    s += a.s_step;
+    at += step;
+    if (s >= a.seq) {
+      s -= a.seq;
+      at += carry;
+    }
+  }
+};
+// Threads of a CTA, by HeadOp: 6 warps (80 registers each) and 5 (96) on each of an SM's four schedulers.
+constexpr int kTileThreads[3] = {768, 768, 640};
+
+template <typename T, int V, bool INTER, int OP>
+__global__ void __launch_bounds__(kTileThreads[OP], 1)
+    heads_tile_kernel(const __grid_constant__ HeadArgs a, unsigned long long limit_ns) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ volatile int abort_flag;
+  constexpr int kBytes = Pack<T, V>::kBytes;
+  constexpr bool NORM = OP != kRotate, BWD = OP == kNormBwd;
+  const HeadSmem lay = head_smem(a, OP, V);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int vecs = a.D / V;
+  uint64_t* freq = reinterpret_cast<uint64_t*>(smem + lay.freq());
+  float* weights = reinterpret_cast<float*>(smem + lay.weight());
+  const uint32_t stage0 = smem_u32(smem), full = smem_u32(smem + lay.bars()), empty = full + 8 * a.stages;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(full + 8 * s, 1 + a.angle_warps);
+      mbar_init(empty + 8 * s, a.groups);
+    }
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) freq[i] = turn_per_step(a.inv_freq[i]);
+  if constexpr (NORM)
     for (int i = threadIdx.x; i < 2 * a.D; i += blockDim.x) {
       const int seg = i >= a.D, d = i - seg * a.D;
-      weights[seg * wstride + d] = load_any(a.w[seg], d, a.wdt);
+      weights[seg * lay.weight_floats + weight_slot<V>(d, vecs)] = load_any(a.w[seg], d, a.wdt);
     }
-    __syncthreads();
-  }
-  const int u = lane & ((1 << a.log_l) - 1), sub = lane >> a.log_l, rpw = 32 >> a.log_l;
-  const bool active = u < a.units;
-  int ia = 0, ib = -1;
-  if (active) unit_vectors<V, INTER>(a, u, ia, ib);
-  const uint32_t items = a.tokens * a.chunks;
-  const int all = a.groups[0] + a.groups[1];
-  for (uint32_t item = blockIdx.x * warps + warp; item < items; item += gridDim.x * warps) {
-    const uint32_t token = item / a.chunks;
-    const uint32_t b = token / a.seq, s = token - b * a.seq;
-    const int g0 = static_cast<int>((item - token * a.chunks) * a.chunk);
-    const int g1 = min(g0 + static_cast<int>(a.chunk), all);
-    __syncwarp();
-    fill_angles(a, cs, b, s, lane);
-    __syncwarp();
-    float2 c[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) c[e] = (active && u < a.rot_units) ? cs[u * V + e] : make_float2(1.f, 0.f);
-    for (int g = g0; g < g1; ++g) {
-      const int seg = g >= a.groups[0];
-      const int head = (g - seg * a.groups[0]) * rpw + sub;
-      const bool ok = active && head < a.heads[seg];
-      float fa[V], fb[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) fa[e] = fb[e] = 0.f;
-      if (ok) {
-        const T* src = static_cast<const T*>(a.x[seg]) + b * a.xs[seg][0] + s * a.xs[seg][1] + head * a.xs[seg][2];
-        Pack<T, V> p;
-        ld_pack(p, src + ia * V);
-        unpack_to<T, V>(p, fa);
-        if (ib >= 0) {
-          ld_pack(p, src + ib * V);
-          unpack_to<T, V>(p, fb);
+  __syncthreads();
+
+  // Wait for a phase; false once any wait of this CTA ran out of time (the loops go on without waiting, so that all
+  // of its warps end).
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (abort_flag) return false;
+    if (mbar_wait(bar, parity, limit_ns)) return true;
+    atomicAdd(&g_heads_timeouts, 1u);
+    abort_flag = 1;
+    return false;
+  };
+
+  if (warp == 0) {  // copies: lane 8 p + k has the k-th token of a tile in q, k, dq, dk (p)
+    const int part = lane >> 3, k = lane & 7, seg = part & 1;
+    const bool mine = part < (BWD ? 4 : 2) && k < a.tt && a.heads[seg] > 0;
+    const bool is_dy = part >= 2;
+    const T* base = static_cast<const T*>(is_dy ? a.dy[seg] : a.x[seg]);
+    const int64_t st_b = is_dy ? a.dys[seg][0] : a.xs[seg][0], st_s = is_dy ? a.dys[seg][1] : a.xs[seg][1];
+    const int64_t st_h = is_dy ? a.dys[seg][2] : a.xs[seg][2];
+    const int64_t step = is_dy ? a.dy_step[seg] : a.x_step[seg], carry = is_dy ? a.dy_carry[seg] : a.x_carry[seg];
+    const bool joined = st_h == a.D || a.heads[seg] == 1;  // heads that follow one another go in one copy
+    const bool all_joined = __all_sync(0xffffffffu, joined || !mine);
+    Place place;
+    uint32_t it = 0, st = 0, phase = 0;
+    for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++it) {
+      const Tile t(a, tile);
+      if (it == 0 || a.parts > 1) place.seek(a, t.token + k, st_b, st_s);
+      else place.next(a, step, carry);
+      const int heads = seg ? t.n[1] : t.n[0];
+      const T* src = base + place.at + (seg ? t.lo[1] : t.lo[0]) * st_h;
+      const uint32_t bar = full + 8 * st;
+      const uint32_t dst = stage0 + st * a.stage_bytes +
+                           ((is_dy ? t.rows[0] + t.rows[1] : 0) + (seg ? t.rows[0] : 0) + k * heads) * a.row_bytes;
+      const bool ok = mine && k < t.count && heads > 0;
+      if (it >= static_cast<uint32_t>(a.stages) && !wait(empty + 8 * st, phase ^ 1u)) break;
+      if (lane == 0) mbar_arrive_expect_tx(bar, (t.rows[0] + t.rows[1]) * a.row_bytes * (BWD ? 2 : 1));
+      __syncwarp();
+      auto copy = [&](uint32_t to, const T* from, int bytes) {
+        asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                     "l"(from), "r"(bytes), "r"(bar)
+                     : "memory");
+      };
+      if (all_joined) {
+        if (ok) copy(dst, src, heads * a.row_bytes);
+      } else {
+        for (int j = 0; j < (BWD ? 32 : 16); ++j) {  // a row a lane, token by token
+          const int n = __shfl_sync(0xffffffffu, ok ? heads : 0, j);
+          const int64_t sh = __shfl_sync(0xffffffffu, st_h, j);
+          const uint32_t to = __shfl_sync(0xffffffffu, dst, j);
+          const T* from = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
+          for (int h = lane; h < n; h += 32) copy(to + h * a.row_bytes, from + h * sh, a.row_bytes);
         }
       }
-      if constexpr (NORM) {
-        float ss = 0.f;
+      if (++st == static_cast<uint32_t>(a.stages)) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+    // no copy is in flight when the CTA ends: the rows' warps wait for every full barrier, or (after a timeout) this does
+    if (abort_flag)
+      for (uint32_t s = 0; s < static_cast<uint32_t>(a.stages) && s < it; ++s)
+        mbar_wait(full + 8 * s, s < st ? phase : phase ^ 1u, limit_ns / 8);
+    return;
+  }
+
+  if (warp <= a.angle_warps) {  // angles, every angle_warps-th token of a tile
+    uint32_t it = 0, st = 0, phase = 0;
+    // this lane's position: axis lane & 3 of the tile's (lane >> 2)-th token of this warp
+    const int mine = warp - 1 + (lane >> 2) * a.angle_warps, axis = lane & 3;
+    Place place;
+    auto position = [&](uint32_t tile, bool seek) {
+      if (tile >= a.tiles) return 0ll;
+      const Tile t(a, tile);
+      if (seek || a.parts > 1) place.seek(a, t.token + mine, a.ps[1], a.ps[2]);
+      else place.next(a, a.p_step, a.p_carry);
+      if (mine >= t.count || axis >= a.axes) return 0ll;
+      const int64_t j = place.at + axis * a.ps[0];
+      return static_cast<long long>(a.pos64 ? static_cast<const int64_t*>(a.pos)[j] : static_cast<const int32_t*>(a.pos)[j]);
+    };
+    // loaded kAhead tiles before their use: a load from HBM takes longer than the angles of a tile
+    constexpr int kAhead = 4;
+    long long ahead[kAhead];
 #pragma unroll
-        for (int e = 0; e < V; ++e) ss += fa[e] * fa[e] + fb[e] * fb[e];
-        const float rstd = rsqrtf(lanes_sum(ss, a.log_l) * a.inv_d + a.eps);
-        const float* w = weights + seg * wstride;
+    for (int q = 0; q < kAhead; ++q) ahead[q] = position(blockIdx.x + q * gridDim.x, q == 0);
+    bool more = true;
+    for (uint32_t tile = blockIdx.x; more;) {
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        if (tile >= a.tiles || (it >= static_cast<uint32_t>(a.stages) && !wait(empty + 8 * st, phase ^ 1u))) {
+          more = false;
+          break;
+        }
+        const int count = Tile(a, tile).count;
+        float2* table = reinterpret_cast<float2*>(smem + lay.angles() + st * lay.angle_bytes);
+        for (int k = warp - 1, j = 0; k < count; k += a.angle_warps, ++j)
+#pragma unroll 2
+          for (int i0 = 0; i0 < a.n; i0 += 32) {
+            const int i = i0 + lane;
+            const int64_t at = __shfl_sync(0xffffffffu, ahead[q], 4 * j + axis_of(a, i));
+            if (i < a.n)
+              table[k * a.n + angle_slot<V>(i, a.rot_units)] = angle_of<sizeof(T) == 4>(at, freq[i], a.sign);
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * st);
+        ahead[q] = position(tile + kAhead * gridDim.x, false);
+        tile += gridDim.x;
+        ++it;
+        if (++st == static_cast<uint32_t>(a.stages)) {
+          st = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    return;
+  }
+
+  // rows
+  const int me = warp - 1 - a.angle_warps;
+  const Lane<INTER> ln(a, lane);
+  const bool rotated = ln.active && ln.u < a.rot_units;
+  const int b_off = (ln.ib - ln.ia) * V, b_bytes = b_off * static_cast<int>(sizeof(T));
+  float da[V], db[V];  // norm backward: dw sums of the tensor in hand; the other's in shared memory
+  float4* other = reinterpret_cast<float4*>(smem + lay.other()) + me * 32 + lane;
+  const int others = a.row_warps * 32;
+  auto exchange = [&] {
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      const float4 f = other[e * others];
+      other[e * others] = make_float4(da[2 * e], da[2 * e + 1], db[2 * e], db[2 * e + 1]);
+      da[2 * e] = f.x;
+      da[2 * e + 1] = f.y;
+      db[2 * e] = f.z;
+      db[2 * e + 1] = f.w;
+    }
+  };
+  bool in_hand = false;
+  if constexpr (BWD) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) da[e] = db[e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) other[e * others] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+
+  // Group g of the CTA's it-th tile: the groups of all its tiles go round the row warps, and a warp waits for those
+  // tiles alone that hold one of its groups. A stage is free when all its groups are done.
+  uint32_t st = 0, phase = 0, tile = blockIdx.x;
+  int g = me;  // row_warps <= groups
+  bool fresh = true;
+  uint32_t base = 0;
+  const float4* table = nullptr;
+  T *out_q = nullptr, *out_k = nullptr;
+  int rows_q = 0, rows_k = 0, q_groups = 0;
+  while (tile < a.tiles) {
+    if (fresh) {
+      const Tile t(a, tile);
+      wait(full + 8 * st, phase);
+      base = stage0 + st * a.stage_bytes;
+      table = reinterpret_cast<const float4*>(smem + lay.angles() + st * lay.angle_bytes);
+      rows_q = t.rows[0];
+      rows_k = t.rows[1];
+      q_groups = (rows_q + a.rpw - 1) / a.rpw;
+      out_q = static_cast<T*>(a.y[0]) + (static_cast<int64_t>(t.token) * a.heads[0] + t.lo[0]) * a.D + ln.ia * V;
+      out_k = static_cast<T*>(a.y[1]) + (static_cast<int64_t>(t.token) * a.heads[1] + t.lo[1]) * a.D + ln.ia * V;
+    }
+    {
+      const bool seg = g >= q_groups;
+      int r = (seg ? g - q_groups : g) * a.rpw + ln.sub;
+      const bool ok = ln.active && r < (seg ? rows_k : rows_q);
+      int row = r + (seg ? rows_q : 0);  // in the stage
+      if (!ok) r = row = 0;
+      if constexpr (BWD)
+        if (seg != in_hand) {
+          exchange();
+          in_hand = seg;
+        }
+      const uint32_t src = base + row * a.row_bytes + ln.ia * kBytes;
+      const uint32_t magic = seg ? a.magic[1] : a.magic[0];
+      const int k = magic ? __umulhi(r, magic) : r;  // the row's token
+      const float4* angles = table + k * (a.n / 2) + ln.u;
+      const int dy_off = (rows_q + rows_k) * a.row_bytes;
+      T* y = (seg ? out_k : out_q) + r * a.D;
+      float xa[V], xb[V];
+      lds_vec<T, V>(src, xa);
+      lds_vec<T, V>(src + b_bytes, xb);
+      if constexpr (!BWD) {
+        if constexpr (NORM) {
+          float sum[1] = {0.f}, sb = 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            sum[0] += xa[e] * xa[e];
+            sb += xb[e] * xb[e];
+          }
+          sum[0] += sb;
+          row_sums(sum, a.units, ln.u, lane);
+          const float rstd = rsqrtf(sum[0] * a.inv_d + a.eps);
+          float w[V];
+          const float* ws = weights + (seg ? lay.weight_floats : 0);
+          read_weights<V>(ws, ln.ia, vecs, w);
+#pragma unroll
+          for (int e = 0; e < V; ++e) xa[e] *= rstd * w[e];
+          read_weights<V>(ws, ln.ib, vecs, w);
+#pragma unroll
+          for (int e = 0; e < V; ++e) xb[e] *= rstd * w[e];
+        }
+        if (rotated) turn<V, INTER>(xa, xb, angles, a.rot_units);
+        if (ok) {
+          st_vec<T, V>(y, xa);
+          st_vec<T, V>(y + b_off, xb);
+        }
+      } else {
+        float ga[V], gb[V], wa[V], wb[V];
+        lds_vec<T, V>(src + dy_off, ga);
+        lds_vec<T, V>(src + dy_off + b_bytes, gb);
+        if (rotated) turn<V, INTER>(ga, gb, angles, a.rot_units);
+        const float* ws = weights + (seg ? lay.weight_floats : 0);
+        read_weights<V>(ws, ln.ia, vecs, wa);
+        read_weights<V>(ws, ln.ib, vecs, wb);
+        float sum[2] = {0.f, 0.f}, sb = 0.f, cb = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          fa[e] *= rstd * w[ia * V + e];
-          if (ib >= 0) fb[e] *= rstd * w[ib * V + e];
+          sum[0] += xa[e] * xa[e];
+          sb += xb[e] * xb[e];
+          wa[e] *= ga[e];
+          wb[e] *= gb[e];
+          sum[1] += wa[e] * xa[e];
+          cb += wb[e] * xb[e];
+        }
+        sum[0] += sb;
+        sum[1] += cb;
+        row_sums(sum, a.units, ln.u, lane);
+        if (ok) {
+          const float rstd = rsqrtf(sum[0] * a.inv_d + a.eps), c = rstd * rstd * (sum[1] * a.inv_d);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            da[e] += ga[e] * (xa[e] * rstd);
+            db[e] += gb[e] * (xb[e] * rstd);
+            wa[e] = rstd * (wa[e] - xa[e] * c);
+            wb[e] = rstd * (wb[e] - xb[e] * c);
+          }
+          st_vec<T, V>(y, wa);
+          st_vec<T, V>(y + b_off, wb);
         }
       }
-      if (ok) {
-        if (u < a.rot_units) rotate_unit<V, INTER>(fa, fb, c, 1.f);
-        T* dst = static_cast<T*>(a.y[seg]) + (static_cast<int64_t>(token) * a.heads[seg] + head) * a.D;
-        st_pack<T, V>(dst + ia * V, fa);
-        if (ib >= 0) st_pack<T, V>(dst + ib * V, fb);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * st);
+    g += a.row_warps;
+    fresh = g >= a.groups;
+    while (g >= a.groups) {
+      g -= a.groups;
+      tile += gridDim.x;
+      if (++st == static_cast<uint32_t>(a.stages)) {
+        st = 0;
+        phase ^= 1u;
       }
     }
   }
-}
 
-// Norm backward: the first q_ctas CTAs walk q's rows, the others k's, so a
-// lane's dw sums (one unit of one weight vector) stay in registers for the
-// whole kernel; they are merged over the CTA in a fixed order into one [D] row
-// of `partial`, which heads_dw_kernel sums over the CTAs, so that the same
-// call gives the same bits.
-template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(256) heads_bwd_kernel(const HeadArgs a) {
-  extern __shared__ __align__(16) float smem_f[];
-  const int wstride = (a.D + 3) & ~3;
-  float* weights = smem_f;                                        // [D]
-  float* sums = smem_f + wstride;                                 // [warps][D]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  float2* cs = reinterpret_cast<float2*>(sums + static_cast<size_t>(warps) * wstride) + static_cast<size_t>(warp) * a.n;
-  const int seg = static_cast<int>(blockIdx.x) >= a.q_ctas;
-  const uint32_t cta = blockIdx.x - (seg ? a.q_ctas : 0), ctas = seg ? gridDim.x - a.q_ctas : a.q_ctas;
-  for (int d = threadIdx.x; d < a.D; d += blockDim.x) weights[d] = load_any(a.w[seg], d, a.wdt);
-  __syncthreads();
-  const int u = lane & ((1 << a.log_l) - 1), sub = lane >> a.log_l, rpw = 32 >> a.log_l;
-  const bool active = u < a.units;
-  int ia = 0, ib = -1;
-  if (active) unit_vectors<V, INTER>(a, u, ia, ib);
-  const uint32_t chunk = seg ? a.chunk_k : a.chunk, chunks = seg ? a.chunks_k : a.chunks;
-  const uint32_t items = a.tokens * chunks;
-  float da[V], db[V];
+  if constexpr (BWD) {
+    // dw: the rows of a group, then the warps (through the stages, which are done with), then (heads_dw_kernel) the CTAs,
+    // each in a fixed order, so that the same call gives the same bits
+    auto rows_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(others) : "memory"); };
+    if (in_hand) exchange();
+    float* sums = reinterpret_cast<float*>(smem + lay.other());
+    float keep[2][2][V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) da[e] = db[e] = 0.f;
-  for (uint32_t item = cta * warps + warp; item < items; item += ctas * warps) {
-    const uint32_t token = item / chunks;
-    const uint32_t b = token / a.seq, s = token - b * a.seq;
-    const int g0 = static_cast<int>((item - token * chunks) * chunk);
-    const int g1 = min(g0 + static_cast<int>(chunk), a.groups[seg]);
-    __syncwarp();
-    fill_angles(a, cs, b, s, lane);
-    __syncwarp();
-    float2 c[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) c[e] = (active && u < a.rot_units) ? cs[u * V + e] : make_float2(1.f, 0.f);
-    for (int g = g0; g < g1; ++g) {
-      const int head = g * rpw + sub;
-      const bool ok = active && head < a.heads[seg];
-      float xa[V], xb[V], ga[V], gb[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) xa[e] = xb[e] = ga[e] = gb[e] = 0.f;
-      if (ok) {
-        const T* src = static_cast<const T*>(a.x[seg]) + b * a.xs[seg][0] + s * a.xs[seg][1] + head * a.xs[seg][2];
-        const T* dsrc = static_cast<const T*>(a.dy[seg]) + b * a.dys[seg][0] + s * a.dys[seg][1] + head * a.dys[seg][2];
-        Pack<T, V> p, q;
-        ld_pack(p, src + ia * V);
-        ld_pack(q, dsrc + ia * V);
-        unpack_to<T, V>(p, xa);
-        unpack_to<T, V>(q, ga);
-        if (ib >= 0) {
-          ld_pack(p, src + ib * V);
-          ld_pack(q, dsrc + ib * V);
-          unpack_to<T, V>(p, xb);
-          unpack_to<T, V>(q, gb);
-        }
-        if (u < a.rot_units) rotate_unit<V, INTER>(ga, gb, c, 1.f);
-      }
-      float wa[V], wb[V], ss = 0.f, cc = 0.f;
+    for (int seg = 0; seg < 2; ++seg) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        wa[e] = weights[ia * V + e];
-        wb[e] = ib >= 0 ? weights[ib * V + e] : 0.f;
-        ss += xa[e] * xa[e] + xb[e] * xb[e];
-        cc += wa[e] * ga[e] * xa[e] + wb[e] * gb[e] * xb[e];
+        float ta = da[e], tb = db[e];
+        for (int r = 1; r < a.rpw; ++r) {
+          ta += __shfl_sync(0xffffffffu, da[e], (ln.u + r * a.units) & 31);
+          tb += __shfl_sync(0xffffffffu, db[e], (ln.u + r * a.units) & 31);
+        }
+        keep[seg][0][e] = ta;
+        keep[seg][1][e] = tb;
       }
-      ss = lanes_sum(ss, a.log_l);
-      cc = lanes_sum(cc, a.log_l);
-      const float rstd = rsqrtf(ss * a.inv_d + a.eps);
-      const float k = rstd * rstd * (cc * a.inv_d);
-      if (ok) {
+      exchange();
+    }
+    rows_sync();  // every lane's own slots are read; they become [row warps][D] sums
+#pragma unroll
+    for (int seg = 0; seg < 2; ++seg) {
+      if (ln.active && ln.sub == 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          da[e] += ga[e] * (xa[e] * rstd);
-          db[e] += gb[e] * (xb[e] * rstd);
-          ga[e] = rstd * (wa[e] * ga[e] - xa[e] * k);
-          gb[e] = rstd * (wb[e] * gb[e] - xb[e] * k);
+          sums[me * a.D + ln.ia * V + e] = keep[seg][0][e];
+          sums[me * a.D + ln.ib * V + e] = keep[seg][1][e];
         }
-        T* dst = static_cast<T*>(a.y[seg]) + (static_cast<int64_t>(token) * a.heads[seg] + head) * a.D;
-        st_pack<T, V>(dst + ia * V, ga);
-        if (ib >= 0) st_pack<T, V>(dst + ib * V, gb);
       }
+      rows_sync();
+      for (int d = me * 32 + lane; d < a.D; d += others) {
+        float t = 0.f;
+        for (int k = 0; k < a.row_warps; ++k) t += sums[k * a.D + d];
+        a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + seg) * a.D + d] = t;
+      }
+      rows_sync();
     }
-  }
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    for (int o = 1 << a.log_l; o < 32; o <<= 1) {
-      da[e] += __shfl_xor_sync(0xffffffffu, da[e], o);
-      db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
-    }
-    if (active && sub == 0) {
-      sums[warp * wstride + ia * V + e] = da[e];
-      if (ib >= 0) sums[warp * wstride + ib * V + e] = db[e];
-    }
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float t = 0.f;
-    for (int k = 0; k < warps; ++k) t += sums[k * wstride + d];
-    a.partial[static_cast<int64_t>(blockIdx.x) * a.D + d] = t;
   }
 }
 
+// A token and one of its groups.
+struct Cursor {
+  uint32_t b, s;
+  int g;
+  DSLPG_DEV Cursor(const HeadArgs& a, int64_t at, int all) {
+    const uint32_t token = static_cast<uint32_t>(at / all);
+    g = static_cast<int>(at - static_cast<int64_t>(token) * all);
+    b = token / a.seq;
+    s = token - b * a.seq;
+  }
+  DSLPG_DEV bool next(const HeadArgs& a, int all) {  // whether a new token begins
+    if (++g < all) return false;
+    g = 0;
+    if (++s == a.seq) {
+      s = 0;
+      ++b;
+    }
+    return true;
+  }
+};
+
 // dw[seg][d] = the sum of the CTAs' partial rows: 8 threads a column, each every 8th row, merged in order.
-__global__ void __launch_bounds__(256) heads_dw_kernel(const float* partial, int q_ctas, int ctas, int D, float* dq,
-                                                       float* dk) {
+__global__ void __launch_bounds__(256) heads_dw_kernel(const float* partial, int ctas, int D, float* dq, float* dk) {
   __shared__ float part[8][32];
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + col, seg = blockIdx.y;
-  const int lo = seg ? q_ctas : 0, hi = seg ? ctas : q_ctas;
   float t = 0.f;
   if (d < D)
-    for (int r = lo + row; r < hi; r += 8) t += partial[static_cast<int64_t>(r) * D + d];
+    for (int r = row; r < ctas; r += 8) t += partial[(static_cast<int64_t>(r) * 2 + seg) * D + d];
   part[row][col] = t;
   __syncthreads();
   if (row == 0 && d < D) {
@@ -344,37 +675,37 @@ __global__ void __launch_bounds__(256) heads_dw_kernel(const float* partial, int
 // scalar accesses, reading it twice (the second time from L1 / L2). `dw` sums
 // are kept per warp in shared memory.
 template <typename T, bool NORM, bool BWD>
-__global__ void __launch_bounds__(128) heads_any_kernel(const HeadArgs a) {
-  extern __shared__ __align__(16) float smem_f[];
+__global__ void __launch_bounds__(128) heads_any_kernel(const __grid_constant__ HeadArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
   const int wstride = (a.D + 3) & ~3;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  float* sums = smem_f + warp * wstride;  // BWD: [warps][D]
-  float2* cs = reinterpret_cast<float2*>(smem_f + (BWD ? warps * wstride : 0)) + static_cast<size_t>(warp) * a.n;
-  const int seg0 = BWD && static_cast<int>(blockIdx.x) >= a.q_ctas;
-  const uint32_t cta = blockIdx.x - (seg0 ? a.q_ctas : 0);
-  const uint32_t ctas = BWD ? (seg0 ? gridDim.x - a.q_ctas : a.q_ctas) : gridDim.x;
-  const int first = BWD ? (seg0 ? a.heads[0] : 0) : 0;
-  const int count = BWD ? a.heads[seg0] : a.heads[0] + a.heads[1];
-  const uint32_t chunk = seg0 ? a.chunk_k : a.chunk, chunks = seg0 ? a.chunks_k : a.chunks;
+  uint64_t* freq = reinterpret_cast<uint64_t*>(smem);                     // [n]
+  float2* cs = reinterpret_cast<float2*>(freq + a.n) + warp * a.n;    // [warps][n]
+  float* all_sums = reinterpret_cast<float*>(smem + 8 * a.n * (warps + 1));
+  float* sums = all_sums + warp * 2 * wstride;                        // BWD: [warps][2][D]
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) freq[i] = turn_per_step(a.inv_freq[i]);
+  __syncthreads();
+  const int all = a.heads[0] + a.heads[1];
+  const int64_t total = static_cast<int64_t>(a.tokens) * all, mine = static_cast<int64_t>(blockIdx.x) * warps + warp;
+  const int64_t share = static_cast<int64_t>(gridDim.x) * warps;
+  const int64_t lo_row = total * mine / share, hi_row = total * (mine + 1) / share;
   if constexpr (BWD)
-    for (int d = lane; d < a.D; d += 32) sums[d] = 0.f;
+    for (int d = lane; d < 2 * wstride; d += 32) sums[d] = 0.f;
   const int n = a.n, D = a.D;
   // Index of the two members of pair i.
   auto lo = [&](int i) { return a.interleaved ? 2 * i : i; };
   auto hi = [&](int i) { return a.interleaved ? 2 * i + 1 : i + n; };
-  const uint32_t items = a.tokens * chunks;
-  for (uint32_t item = cta * warps + warp; item < items; item += ctas * warps) {
-    const uint32_t token = item / chunks;
-    const uint32_t b = token / a.seq, s = token - b * a.seq;
-    const int h0 = static_cast<int>((item - token * chunks) * chunk);
-    const int h1 = min(h0 + static_cast<int>(chunk), count);
-    __syncwarp();
-    fill_angles(a, cs, b, s, lane);
-    __syncwarp();
-    for (int h = first + h0; h < first + h1; ++h) {
-      const int seg = h >= a.heads[0], head = h - (seg ? a.heads[0] : 0);
+  if (hi_row > lo_row) {
+    Cursor at(a, lo_row, all);
+    bool fresh = true;
+    for (int64_t row = lo_row; row < hi_row; ++row, fresh = at.next(a, all)) {
+      const uint32_t b = at.b, s = at.s;
+      if (fresh) {
+        fill_angles<sizeof(T) == 4>(a, freq, cs, lane_position(a, b * a.ps[1] + s * a.ps[2], lane), lane);
+      }
+      const int seg = at.g >= a.heads[0], head = at.g - (seg ? a.heads[0] : 0);
       const T* src = static_cast<const T*>(a.x[seg]) + b * a.xs[seg][0] + s * a.xs[seg][1] + head * a.xs[seg][2];
-      T* dst = static_cast<T*>(a.y[seg]) + (static_cast<int64_t>(token) * a.heads[seg] + head) * D;
+      T* dst = static_cast<T*>(a.y[seg]) + ((static_cast<int64_t>(b) * a.seq + s) * a.heads[seg] + head) * D;
       float rstd = 1.f;
       if constexpr (NORM) {
         float ss = 0.f;
@@ -410,7 +741,7 @@ __global__ void __launch_bounds__(128) heads_any_kernel(const HeadArgs a) {
         const float k = rstd * rstd * (warp_reduce<SumOp>(cc) * a.inv_d);
         auto put = [&](int d, float g) {
           const float v = to_f(src[d]);
-          sums[d] += g * (v * rstd);  // feature d is the same lane's in every row
+          sums[seg * wstride + d] += g * (v * rstd);  // feature d is the same lane's in every row
           dst[d] = from_f<T>(rstd * (w(d) * g - v * k));
         };
         for (int i = lane; i < n; i += 32) {
@@ -425,10 +756,11 @@ __global__ void __launch_bounds__(128) heads_any_kernel(const HeadArgs a) {
   }
   if constexpr (BWD) {
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+      const int seg = i >= D, d = i - seg * D;
       float t = 0.f;
-      for (int k = 0; k < warps; ++k) t += smem_f[k * wstride + d];
-      a.partial[static_cast<int64_t>(blockIdx.x) * D + d] = t;
+      for (int k = 0; k < warps; ++k) t += all_sums[(2 * k + seg) * wstride + d];
+      a.partial[static_cast<int64_t>(blockIdx.x) * 2 * D + i] = t;
     }
   }
 }
@@ -436,132 +768,132 @@ __global__ void __launch_bounds__(128) heads_any_kernel(const HeadArgs a) {
 namespace {
 
 constexpr int kMaxHeadDim = 1024;
-constexpr int kPartialRows = 1184;  // CTAs of a norm backward at most (8 for each of 148 SMs)
+constexpr int kPartialRows = 1184;  // CTAs of a norm backward at most (8 for each of 148 SMs), each with a row for q and one for k
 
-// Groups of heads a warp takes per item: all of a token's, fewer while that leaves warps without work.
-uint32_t chunk_of(int groups, uint32_t tokens, int64_t warps) {
-  int64_t chunk = groups;
-  while (chunk > 1 && static_cast<int64_t>(tokens) * ((groups + chunk - 1) / chunk) < warps) chunk = (chunk + 1) / 2;
-  return static_cast<uint32_t>(chunk < 1 ? 1 : chunk);
+constexpr int kTileSmem = 216 * 1024;  // of the 227 KB that a CTA may have
+constexpr int kAnyBlock = 128;
+
+uint32_t magic_of(int heads) { return heads > 1 ? static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads) : 0; }
+
+// Cut the work into tiles. A tile holds up to 8 tokens and 80 KB (rotation alone:
+// 40 KB), fewer tokens while that leaves SMs without four tiles each, and less
+// than a token where one token is too large or there are not tokens enough.
+// Measured (us) with 20, 40 and 80 KB: norm forward of 16384 tokens of 32 + 8
+// heads of 128 in bf16 90.2, 61.6, 59.5 (its backward 147, 113, 107); rotation of
+// 29971 tokens of 16 + 16 heads 135, 86.0, 90.8.
+template <typename T> void set_tiles(HeadArgs& a, int op) {
+  const int heads = a.heads[0] + a.heads[1], copies = op == kNormBwd ? 2 : 1, sms = sm_count();
+  a.row_bytes = a.D * static_cast<int>(sizeof(T));
+  const int64_t row = static_cast<int64_t>(a.row_bytes) * copies, token = row * heads;
+      const int64_t want = (op == kRotate ? 40 : 80) * 1024;
+  a.parts = 1;
+  a.part = heads;
+  a.tt = 1;
+  while (a.tt < kMaxTileTokens && token * a.tt * 2 <= want && static_cast<int64_t>(a.tokens) >= 4ll * a.tt * sms) a.tt *= 2;
+  if (a.tt == 1) {
+    // at most 32 KB of rows, and as many parts as leave every SM one, but whole groups of rows
+    int64_t part = heads;
+    if (token > 32 * 1024) part = 32 * 1024 / row;
+    const int64_t spare = (sms + static_cast<int64_t>(a.tokens) - 1) / a.tokens;
+    if (heads / spare < part) part = heads / spare;
+    part = part < 1 ? a.rpw : (part + a.rpw - 1) / a.rpw * a.rpw;
+    if (part < heads) {
+      a.part = static_cast<int>(part);
+      a.parts = (heads + a.part - 1) / a.part;
+    }
+  }
+  a.tiles = a.parts == 1 ? (a.tokens + a.tt - 1) / a.tt : a.tokens * a.parts;
+  a.stage_bytes = static_cast<int>((row * (a.parts == 1 ? static_cast<int64_t>(heads) * a.tt : a.part) + 127) & ~127ll);
+  a.magic[0] = a.parts == 1 ? magic_of(a.heads[0]) : magic_of(1 << 30);
+  a.magic[1] = a.parts == 1 ? magic_of(a.heads[1]) : magic_of(1 << 30);
 }
 
-template <typename K>
-int grid_for(K kernel, int block, size_t smem, int64_t items, cudaError_t& e) {
-  const void* fn = reinterpret_cast<const void*>(kernel);
-  if (smem > 48 * 1024 && (e = allow_dynamic_smem(fn, smem)) != cudaSuccess) return 0;
-  return persistent_grid(fn, block, smem, (items + block / 32 - 1) / (block / 32));
-}
-
-// The q : k split of a norm backward's CTAs, by their groups.
-int split_ctas(const HeadArgs& a, int grid) {
-  const int64_t all = a.groups[0] + a.groups[1];
-  if (a.groups[1] == 0) return grid;
-  int64_t q = (static_cast<int64_t>(grid) * a.groups[0] + all / 2) / all;
-  if (a.groups[0] > 0 && q < 1) q = 1;
-  if (q > grid - 1) q = grid - 1;
-  return static_cast<int>(q);
-}
-
-template <typename T, int V, bool INTER, bool NORM>
-cudaError_t launch_fwd(HeadArgs a, cudaStream_t st) {
-  const int block = 256;
-  const size_t smem = (NORM ? 2 * ((a.D + 3) & ~3) * 4 : 0) + static_cast<size_t>(block / 32) * a.n * 8;
-  const int all = a.groups[0] + a.groups[1];
-  a.chunk = chunk_of(all, a.tokens, static_cast<int64_t>(sm_count()) * 16);
-  a.chunks = (all + a.chunk - 1) / a.chunk;
-  cudaError_t e = cudaSuccess;
-  const int grid = grid_for(&heads_fwd_kernel<T, V, INTER, NORM>, block, smem, static_cast<int64_t>(a.tokens) * a.chunks, e);
-  if (e != cudaSuccess) return e;
-  heads_fwd_kernel<T, V, INTER, NORM><<<grid, block, smem, st>>>(a);
+template <typename T, int V, bool INTER, int OP>
+cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
+  a.rot_units = a.n / V;
+  a.units = a.D / (2 * V);
+  a.rpw = 32 / a.units;
+  set_tiles<T>(a, OP);
+  a.groups = a.parts == 1 ? (a.heads[0] * a.tt + a.rpw - 1) / a.rpw + (a.heads[1] * a.tt + a.rpw - 1) / a.rpw
+                          : (a.part + a.rpw - 1) / a.rpw + 1;
+  // Warps: one for copies; some for angles; the rest for rows, no more than a tile has groups. One angle warp for two
+  // tokens (backward, whose rows take twice the time: for four; 107.4 us against 110.7 for the training batch above).
+  a.angle_warps = OP == kNormBwd ? (a.tt + 3) / 4 : (a.tt + 1) / 2;
+  a.row_warps = kTileThreads[OP] / 32 - 1 - a.angle_warps;
+  if (a.row_warps > a.groups) a.row_warps = a.groups;
+  const int block = 32 * (1 + a.angle_warps + a.row_warps);
+  const void* fn = reinterpret_cast<const void*>(&heads_tile_kernel<T, V, INTER, OP>);
+  const int grid = static_cast<int>(a.tiles < static_cast<uint32_t>(sm_count()) ? a.tiles : sm_count());
+  const int mine = static_cast<int>((a.tiles + grid - 1) / grid);  // tiles of a CTA at most
+  for (a.stages = mine < 16 ? mine : 16; a.stages > 1 && head_smem(a, OP, V).total() > kTileSmem; --a.stages) {
+  }
+  const int64_t ahead = static_cast<int64_t>(grid) * a.tt, db = ahead / a.seq, ds = ahead % a.seq;
+  for (int seg = 0; seg < 2; ++seg) {
+    a.x_step[seg] = db * a.xs[seg][0] + ds * a.xs[seg][1];
+    a.x_carry[seg] = a.xs[seg][0] - static_cast<int64_t>(a.seq) * a.xs[seg][1];
+    a.dy_step[seg] = db * a.dys[seg][0] + ds * a.dys[seg][1];
+    a.dy_carry[seg] = a.dys[seg][0] - static_cast<int64_t>(a.seq) * a.dys[seg][1];
+  }
+  a.p_step = db * a.ps[1] + ds * a.ps[2];
+  a.p_carry = a.ps[1] - static_cast<int64_t>(a.seq) * a.ps[2];
+  a.s_step = static_cast<uint32_t>(ds);
+  const size_t smem = head_smem(a, OP, V).total();
+  if (cudaError_t e = allow_dynamic_smem(fn, smem)) return e;
+  heads_tile_kernel<T, V, INTER, OP><<<grid, block, smem, st>>>(a, kWaitLimitNs);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  if constexpr (OP == kNormBwd) heads_dw_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, grid, a.D, dwq, dwk);
   return cudaGetLastError();
-}
-
-template <typename K>
-cudaError_t launch_bwd_with(K kernel, HeadArgs a, int block, size_t smem, float* dwq, float* dwk, cudaStream_t st) {
-  const int64_t want = static_cast<int64_t>(sm_count()) * 16;
-  a.chunk = chunk_of(a.groups[0], a.tokens, want);
-  a.chunks = (a.groups[0] + a.chunk - 1) / a.chunk;
-  a.chunk_k = chunk_of(a.groups[1], a.tokens, want);
-  a.chunks_k = (a.groups[1] + a.chunk_k - 1) / a.chunk_k;
-  cudaError_t e = cudaSuccess;
-  int grid = grid_for(kernel, block, smem, static_cast<int64_t>(a.tokens) * (a.chunks + a.chunks_k), e);
-  if (e != cudaSuccess) return e;
-  if (grid > kPartialRows) grid = kPartialRows;
-  if (grid < 2) grid = 2;
-  a.q_ctas = split_ctas(a, grid);
-  kernel<<<grid, block, smem, st>>>(a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  heads_dw_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, a.q_ctas, grid, a.D, dwq, dwk);
-  return cudaGetLastError();
-}
-
-template <typename T, int V, bool INTER>
-cudaError_t launch_bwd(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
-  const int block = 256, ws = (a.D + 3) & ~3;
-  const size_t smem = static_cast<size_t>(ws) * 4 * (1 + block / 32) + static_cast<size_t>(block / 32) * a.n * 8;
-  return launch_bwd_with(&heads_bwd_kernel<T, V, INTER>, a, block, smem, dwq, dwk, st);
 }
 
 template <typename T, bool NORM, bool BWD>
 cudaError_t launch_any(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
-  const int block = 128, ws = (a.D + 3) & ~3;
-  const size_t smem = (BWD ? static_cast<size_t>(ws) * 4 * (block / 32) : 0) + static_cast<size_t>(block / 32) * a.n * 8;
-  a.groups[0] = a.heads[0];
-  a.groups[1] = a.heads[1];
-  if constexpr (BWD) {
-    return launch_bwd_with(&heads_any_kernel<T, NORM, true>, a, block, smem, dwq, dwk, st);
-  } else {
-    const int all = a.heads[0] + a.heads[1];
-    a.chunk = chunk_of(all, a.tokens, static_cast<int64_t>(sm_count()) * 16);
-    a.chunks = (all + a.chunk - 1) / a.chunk;
-    cudaError_t e = cudaSuccess;
-    const int grid =
-        grid_for(&heads_any_kernel<T, NORM, false>, block, smem, static_cast<int64_t>(a.tokens) * a.chunks, e);
-    if (e != cudaSuccess) return e;
-    heads_any_kernel<T, NORM, false><<<grid, block, smem, st>>>(a);
-    return cudaGetLastError();
-  }
+  const size_t smem = (BWD ? static_cast<size_t>((a.D + 3) & ~3) * 8 * (kAnyBlock / 32) : 0) +
+                      static_cast<size_t>(kAnyBlock / 32 + 1) * a.n * 8;
+  const void* fn = reinterpret_cast<const void*>(&heads_any_kernel<T, NORM, BWD>);
+  if (cudaError_t e = allow_dynamic_smem(fn, smem)) return e;
+  const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads[0] + a.heads[1]);
+  int grid = persistent_grid(fn, kAnyBlock, smem, (rows + kAnyBlock / 32 - 1) / (kAnyBlock / 32));
+  if (BWD && grid > kPartialRows) grid = kPartialRows;
+  heads_any_kernel<T, NORM, BWD><<<grid, kAnyBlock, smem, st>>>(a);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  if constexpr (BWD) heads_dw_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, grid, a.D, dwq, dwk);
+  return cudaGetLastError();
 }
 
-// Whether rows can be cut into units of two V-element vectors: sizes, strides and bases.
+// Whether rows can be cut into units of two V-element vectors.
 template <typename T>
-bool fits(const HeadArgs& a, int V, bool bwd) {
-  if (a.D % V || a.n % V) return false;  // n % V: half of the rotated features, or 2 V of them interleaved
-  const int units = a.n / V + (a.D / V - 2 * (a.n / V) + 1) / 2;
-  if (units > 32) return false;
-  const int bytes = V * static_cast<int>(sizeof(T));
+bool fits(const HeadArgs& a, int V) {
+  // n % V: half of the rotated features, or 2 V of them interleaved; the others in pairs of vectors too
+  return a.D % (2 * V) == 0 && a.n % V == 0 && a.D / (2 * V) <= 32;
+}
+
+// Whether rows can be copied in bulk: 16-byte addresses and sizes.
+template <typename T>
+bool copies_fit(const HeadArgs& a, bool bwd) {
+  constexpr int E = Elt<T>::kPerVec;
+  if (a.D % E) return false;
   for (int seg = 0; seg < 2; ++seg) {
-    if (!aligned(a.x[seg], bytes) || !aligned(a.y[seg], bytes) || (bwd && !aligned(a.dy[seg], bytes))) return false;
+    if (!aligned(a.x[seg], 16) || !aligned(a.y[seg], 16) || (bwd && !aligned(a.dy[seg], 16))) return false;
     for (int k = 0; k < 3; ++k)
-      if (a.xs[seg][k] % V || (bwd && a.dys[seg][k] % V)) return false;
+      if (a.xs[seg][k] % E || (bwd && a.dys[seg][k] % E)) return false;
   }
   return true;
 }
 
-void set_units(HeadArgs& a, int V) {
-  a.rot_units = a.n / V;
-  a.units = a.rot_units + (a.D / V - 2 * a.rot_units + 1) / 2;
-  a.log_l = 0;
-  while ((1 << a.log_l) < a.units) ++a.log_l;
-  const int rpw = 32 >> a.log_l;
-  for (int seg = 0; seg < 2; ++seg) a.groups[seg] = (a.heads[seg] + rpw - 1) / rpw;
-}
-
 template <typename T, int V, bool INTER>
-cudaError_t launch_v(HeadArgs a, bool norm, bool bwd, float* dwq, float* dwk, cudaStream_t st) {
-  set_units(a, V);
-  if (bwd) return launch_bwd<T, V, INTER>(a, dwq, dwk, st);
-  return norm ? launch_fwd<T, V, INTER, true>(a, st) : launch_fwd<T, V, INTER, false>(a, st);
+cudaError_t launch_v(const HeadArgs& a, bool norm, bool bwd, float* dwq, float* dwk, cudaStream_t st) {
+  if (bwd) return launch_tile<T, V, INTER, kNormBwd>(a, dwq, dwk, st);
+  return norm ? launch_tile<T, V, INTER, kNorm>(a, dwq, dwk, st) : launch_tile<T, V, INTER, kRotate>(a, dwq, dwk, st);
 }
 
 template <typename T>
 cudaError_t dispatch(HeadArgs a, bool norm, bool bwd, float* dwq, float* dwk, cudaStream_t st) {
   constexpr int E = Elt<T>::kPerVec;
-  if (kernel_path() != DSLPG_PATH_STREAM) {
-    if (fits<T>(a, E, bwd))
+  if (kernel_path() != DSLPG_PATH_STREAM && copies_fit<T>(a, bwd)) {
+    if (fits<T>(a, E))
       return a.interleaved ? launch_v<T, E, true>(a, norm, bwd, dwq, dwk, st)
                            : launch_v<T, E, false>(a, norm, bwd, dwq, dwk, st);
-    if (fits<T>(a, E / 2, bwd))
+    if (fits<T>(a, E / 2))
       return a.interleaved ? launch_v<T, E / 2, true>(a, norm, bwd, dwq, dwk, st)
                            : launch_v<T, E / 2, false>(a, norm, bwd, dwq, dwk, st);
   }
@@ -618,6 +950,7 @@ int common_args(HeadArgs& a, const dslpg_heads* h, const void* positions, const 
     a.dys[1][k] = extents[1][k] > 1 ? h->dk_strides[k] : 0;
     a.ps[k] = pos_extents[k] > 1 ? h->position_strides[k] : 0;
   }
+  a.axes = h->axes;
   a.pos64 = h->positions_dtype == DSLPG_I64 ? 1 : 0;
   a.interleaved = h->interleaved ? 1 : 0;
   a.inv_d = 1.0f / static_cast<float>(a.D);
@@ -648,6 +981,14 @@ int run_rope(const void* q, const void* k, const void* positions, const float* i
 }
 
 }  // namespace
+
+unsigned int take_wait_timeouts_heads() {
+  unsigned int v = 0, zero = 0;
+  cudaMemcpyFromSymbol(&v, g_heads_timeouts, sizeof(v));
+  cudaMemcpyToSymbol(g_heads_timeouts, &zero, sizeof(zero));
+  return v;
+}
+
 }  // namespace dslpg
 
 using namespace dslpg;
@@ -686,7 +1027,7 @@ extern "C" int dslpg_qk_norm_rope_fwd(const void* q, const void* k, const void* 
 extern "C" int dslpg_qk_norm_rope_bwd_workspace_bytes(int64_t head_dim, int64_t* bytes) {
   if (!bytes) return DSLPG_ERR_NULL_POINTER;
   if (head_dim < 1 || head_dim > kMaxHeadDim) return DSLPG_ERR_BAD_SHAPE;
-  *bytes = kPartialRows * head_dim * 4;
+  *bytes = kPartialRows * 2 * head_dim * 4;
   return DSLPG_OK;
 }
 
@@ -700,7 +1041,7 @@ extern "C" int dslpg_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, co
   if (int rc = common_args(a, h, positions, inv_freq, -1.f)) return rc;
   if (!is_float_dtype(h->weight_dtype)) return DSLPG_ERR_BAD_DTYPE;
   if (!eps_ok(eps)) return DSLPG_ERR_BAD_EPS;
-  if (workspace_bytes < static_cast<int64_t>(kPartialRows) * a.D * 4 || !aligned(workspace, 16)) return DSLPG_ERR_BAD_ARGUMENT;
+  if (workspace_bytes < static_cast<int64_t>(kPartialRows) * 2 * a.D * 4 || !aligned(workspace, 16)) return DSLPG_ERR_BAD_ARGUMENT;
   if (a.tokens == 0 || a.heads[0] + a.heads[1] == 0) {
     cudaError_t e = cudaMemsetAsync(dq_weight, 0, static_cast<size_t>(a.D) * 4, stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(dk_weight, 0, static_cast<size_t>(a.D) * 4, stream);
