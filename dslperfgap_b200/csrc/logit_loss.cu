@@ -25,6 +25,7 @@
 // direction (some 2e-7), which a sum over a sequence's rows adds up. Both parts
 // have one sign, so that a logit of -inf gives d = -inf and not NaN.
 #include "common.cuh"
+#include "pipe.cuh"
 
 namespace dslpg {
 
@@ -36,8 +37,7 @@ struct LossRows {
   double scale;
   float scale_f, sign;  // scale as float32; 1 or -1
   float c_hi, c_lo;     // scale * log2(e) in two parts of one sign
-  int tpr, rpc;         // threads of a row, rows of a CTA (statistics kernel)
-  int nvec;             // N / V on the vector path
+  int tpr, rpc;         // threads of a row, rows of a CTA
 };
 
 struct PolicyTerms {
@@ -196,95 +196,142 @@ DSLPG_DEV float pair_slope(const PairTerms& p, const float* log_ratio, int64_t s
 
 enum LossKind : int { kPolicy = 0, kPair = 1 };
 
-// Fold a whole row with `tpr` threads, this one being t: 16-byte vectors
-// (V > 1), the next ones loaded before this round's arithmetic, or scalars.
-template <typename T, int V, int U, class Load>
-DSLPG_DEV void fold_row(Stat& st, const T* xr, const LossRows& a, int t, int tpr, Load ld) {
-  if constexpr (V > 1) {
-    const int stride = U * tpr;
-    auto load = [&](Vec16 (&dst)[U], int j0) {
+// A stretch of n elements from p on as vectors: `head` elements up to the next
+// 16-byte boundary, `vecs` vectors, and `tail` elements.
+template <typename T> struct Stretch {
+  int head, vecs, tail;
+  DSLPG_DEV Stretch(const T* p, int64_t n) {
+    constexpr int E = Elt<T>::kPerVec;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / static_cast<int>(sizeof(T));
+    const int64_t h = off ? E - off : 0;
+    head = static_cast<int>(h < n ? h : n);
+    vecs = static_cast<int>((n - head) / E);
+    tail = static_cast<int>(n - head - static_cast<int64_t>(vecs) * E);
+  }
+};
+
+// Fold elements [0, n) from xr on with `tpr` threads, this one being t: 16-byte
+// vectors, the next ones loaded before this round's arithmetic, and the elements
+// before the first and behind the last whole vector, one a thread.
+template <typename T, int U, class Load>
+DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int t, int tpr, Load ld) {
+  constexpr int E = Elt<T>::kPerVec;
+  const Stretch<T> w(xr, n);
+  const T* body = xr + w.head;
+  const int stride = U * tpr;
+  auto load = [&](Vec16 (&dst)[U], int j0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * tpr;
+      dst[u] = Vec16{{0u, 0u, 0u, 0u}};
+      if (j < w.vecs) dst[u] = ld(body + static_cast<int64_t>(j) * E);
+    }
+  };
+  Vec16 nx[U];
+  load(nx, t);
+  if (t < w.head + w.tail) {
+    const float x[1] = {to_f(t < w.head ? xr[t] : xr[n - w.tail + (t - w.head)])};
+    const bool ok[1] = {true};
+    fold_values<1>(st, x, ok, a);
+  }
+  for (int j0 = t; j0 < w.vecs; j0 += stride) {
+    Vec16 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = nx[u];
+    if (j0 + stride < w.vecs) load(nx, j0 + stride);
+    if (j0 + (U - 1) * tpr < w.vecs) {
+      fold_rows<T, U>(st, v, a);
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = j0 + u * tpr;
-        dst[u] = Vec16{{0u, 0u, 0u, 0u}};
-        if (j < a.nvec) dst[u] = ld(xr + static_cast<int64_t>(j) * V);
-      }
-    };
-    Vec16 nx[U];
-    load(nx, t);
-    for (int j0 = t; j0 < a.nvec; j0 += stride) {
-      Vec16 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = nx[u];
-      if (j0 + stride < a.nvec) load(nx, j0 + stride);
-      if (j0 + (U - 1) * tpr < a.nvec) {
-        fold_rows<T, U>(st, v, a);
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (j0 + u * tpr < a.nvec) {
-            const Vec16 one[1] = {v[u]};
-            fold_rows<T, 1>(st, one, a);
-          }
+        if (j0 + u * tpr < w.vecs) {
+          const Vec16 one[1] = {v[u]};
+          fold_rows<T, 1>(st, one, a);
         }
       }
-    }
-  } else {
-    constexpr int W = 8;
-    for (int64_t j0 = t; j0 < a.N; j0 += static_cast<int64_t>(W) * tpr) {
-      float x[W];
-      bool ok[W];
-#pragma unroll
-      for (int u = 0; u < W; ++u) {
-        const int64_t j = j0 + static_cast<int64_t>(u) * tpr;
-        ok[u] = j < a.N;
-        x[u] = ok[u] ? to_f(xr[j]) : 0.f;
-      }
-      fold_values<W>(st, x, ok, a);
     }
   }
 }
 
+// The results of a row that counts, or of one that is left out.
+template <int KIND>
+DSLPG_DEV void write_row(const LossRows& a, const PolicyTerms& pol, const LossOut& o, int64_t r, bool counts, float xl,
+                         float gm, float gs) {
+  double logp = 0.0, lse = 0.0;
+  PolicyRow p{0.f, 0.f, 0.f};
+  if (counts) {
+    const RowStat rs(gm, gs, a);
+    lse = rs.lse(a);
+    logp = rs.logp(a, xl);
+    if constexpr (KIND == kPolicy) p = policy_row(pol, r, logp);
+  }
+  o.logp[r] = static_cast<float>(logp);
+  o.lse[r] = static_cast<float>(lse);
+  if constexpr (KIND == kPolicy) {
+    o.loss[r] = p.loss;
+    o.kl[r] = p.kl;
+  }
+}
+
+template <int KIND> DSLPG_DEV int64_t counted_col(const LossRows& a, const PairTerms& pair, int64_t r) {
+  int64_t col = label_col(a, r);
+  if constexpr (KIND == kPair)
+    if (col >= 0 && sequence_of(pair, r, a.M) < 0) col = -1;
+  return col;
+}
+
 // Row statistics: `tpr` threads a row. Writes the row's losses (policy) or its
 // logp and lse (preferences; pair_kernel then sums them).
-template <int KIND, typename T, int V>
-__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const LossRows a, const PolicyTerms pol, const PairTerms pair,
-                                                           const LossOut o) {
+template <int KIND, typename T>
+__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant__ LossRows a,
+                                                           const __grid_constant__ PolicyTerms pol,
+                                                           const __grid_constant__ PairTerms pair, const LossOut o) {
   __shared__ float red[2][32];
   const int g = threadIdx.x / a.tpr, t = threadIdx.x - g * a.tpr;
   const int nw = a.tpr >> 5, first_warp = g * nw;
   const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.rpc; base < a.M; base += step) {
     const int64_t r = base + g;
-    int64_t col = r < a.M ? label_col(a, r) : -1;
-    if constexpr (KIND == kPair)
-      if (col >= 0 && sequence_of(pair, r, a.M) < 0) col = -1;
+    const int64_t col = r < a.M ? counted_col<KIND>(a, pair, r) : -1;
     const T* xr = static_cast<const T*>(a.x) + r * a.ld;
     Stat st;
     float xl = 0.f;
     if (col >= 0) {
       if (t == 0) xl = to_f(xr[col]);
-      fold_row<T, V, 4>(st, xr, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      fold_row<T, 4>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
     }
     const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
     const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
-    if (t == 0 && r < a.M) {
-      double logp = 0.0, lse = 0.0;
-      PolicyRow p{0.f, 0.f, 0.f};
-      if (col >= 0) {
-        const RowStat rs(gm, gs, a);
-        lse = rs.lse(a);
-        logp = rs.logp(a, xl);
-        if constexpr (KIND == kPolicy) p = policy_row(pol, r, logp);
-      }
-      o.logp[r] = static_cast<float>(logp);
-      o.lse[r] = static_cast<float>(lse);
-      if constexpr (KIND == kPolicy) {
-        o.loss[r] = p.loss;
-        o.kl[r] = p.kl;
-      }
-    }
+    if (t == 0 && r < a.M) write_row<KIND>(a, pol, o, r, col >= 0, xl, gm, gs);
   }
+}
+
+// The same for few long rows: a cluster of CTAs a row, each folding a stretch of
+// it; their statistics meet in distributed shared memory.
+template <int KIND, typename T>
+__global__ void __launch_bounds__(512) loss_split_kernel(const __grid_constant__ LossRows a,
+                                                         const __grid_constant__ PolicyTerms pol,
+                                                         const __grid_constant__ PairTerms pair, const LossOut o) {
+  __shared__ float red[2][32];
+  __shared__ float slots[2];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+  const int64_t r = blockIdx.x / C;
+  const int64_t col = counted_col<KIND>(a, pair, r);
+  ClusterReducer rd{slots, red, 0, C};
+  Stat st;
+  float xl = 0.f;
+  if (col >= 0) {
+    const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+    const int64_t part = ((a.N + C - 1) / C + 63) & ~63ll, lo = part * rank, n = lo + part < a.N ? part : a.N - lo;
+    if (threadIdx.x == 0 && rank == 0) xl = to_f(xr[col]);
+    if (n > 0) fold_row<T, 4>(st, xr + lo, n, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
+  }
+  const float gm = rd.template reduce<MaxOp>(st.m);
+  const float gs = rd.template reduce<SumOp>(merged(st, gm, a));
+  if (rank == 0 && threadIdx.x == 0) write_row<KIND>(a, pol, o, r, col >= 0, xl, gm, gs);
+  cl.sync();  // no CTA leaves while another may still read its slots
 }
 
 DSLPG_DEV double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
@@ -327,80 +374,157 @@ struct GradTerms {
   float k1, shift, c, off;
 };
 
-// dlogits of one row by `nt` threads, then the label column, k1 expm1(logp).
-// The next chunk's loads are issued before this chunk's arithmetic.
-template <typename T, int V, int U>
-DSLPG_DEV void grad_row(const T* xr, T* yr, const LossRows& a, const GradTerms& gt, double logp, int64_t col, int t,
-                        int nt) {
-  if constexpr (V > 1) {
-    constexpr int P = Elt<T>::kPerVec / 2;
+// p = 2^((x + shift) c + off) times k1 for the elements of a vector.
+template <typename T> DSLPG_DEV void grad_vec(const Vec16& v, const GradTerms& gt, T* dst) {
+  constexpr int P = Elt<T>::kPerVec / 2;
+  const f32x2 c2 = pk2(gt.c, gt.c), sh2 = pk2(gt.shift, gt.shift), off2 = pk2(gt.off, gt.off), k2 = pk2(gt.k1, gt.k1);
+  f32x2 y[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    float d0, d1;
+    upk2(fma2(add2(unpack_pair<T>(v, p), sh2), c2, off2), d0, d1);
+    y[p] = mul2(k2, pk2(ex2(d0), ex2(d1)));
+  }
+  StorePairs<T, P>::run(dst, y);
+}
+
+template <typename T> DSLPG_DEV void grad_one(const T* x, T* y, const GradTerms& gt) {
+  *y = from_f<T>(gt.k1 * ex2(fmaf(to_f(*x) + gt.shift, gt.c, gt.off)));
+}
+
+// 16 bytes from any element on: the two vectors around them, shifted together.
+// `s`: their distance from a 16-byte boundary (the same for a whole row).
+DSLPG_DEV Vec16 shifted_vec(const Vec16& lo, const Vec16& hi, int s) {
+  uint32_t w[8] = {lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]};
+  if (s & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  Vec16 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.w[i] = __funnelshift_r(w[i], w[i + 1], (s & 3) * 8);
+  return v;
+}
+
+// dlogits of elements [0, n) by `nt` threads, this one being t, then the label
+// column (col, if in there): k1 expm1(logp). Vectors are those of the output; the
+// logits' may lie at another distance from a 16-byte boundary (rows of odd
+// length). The next chunk's loads are issued before this chunk's arithmetic.
+template <typename T, int U>
+DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
+  constexpr int E = Elt<T>::kPerVec;
+  const Stretch<T> w(yr, n);
+  const T* xb = xr + w.head;
+  T* yb = yr + w.head;
+  const int s = static_cast<int>(reinterpret_cast<uintptr_t>(xb) & 15);
+  if (s == 0) {
     auto load = [&](Vec16 (&dst)[U], int j0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * nt;
         dst[u] = Vec16{{0u, 0u, 0u, 0u}};
-        if (j < a.nvec) dst[u] = ld_stream(xr + static_cast<int64_t>(j) * V);
+        if (j < w.vecs) dst[u] = ld_stream(xb + static_cast<int64_t>(j) * E);
       }
     };
-    const f32x2 c2 = pk2(gt.c, gt.c), sh2 = pk2(gt.shift, gt.shift), off2 = pk2(gt.off, gt.off), k2 = pk2(gt.k1, gt.k1);
     Vec16 nx[U];
     load(nx, t);
-    for (int j0 = t; j0 < a.nvec; j0 += U * nt) {
+    for (int j0 = t; j0 < w.vecs; j0 += U * nt) {
       Vec16 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = nx[u];
-      if (j0 + U * nt < a.nvec) load(nx, j0 + U * nt);
+      if (j0 + U * nt < w.vecs) load(nx, j0 + U * nt);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * nt;
-        if (j >= a.nvec) continue;
-        f32x2 y[P];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          float d0, d1;
-          upk2(fma2(add2(unpack_pair<T>(v[u], p), sh2), c2, off2), d0, d1);
-          y[p] = mul2(k2, pk2(ex2(d0), ex2(d1)));
-        }
-        StorePairs<T, P>::run(yr + static_cast<int64_t>(j) * V, y);
+        if (j < w.vecs) grad_vec<T>(v[u], gt, yb + static_cast<int64_t>(j) * E);
       }
     }
   } else {
-    for (int64_t j = t; j < a.N; j += nt) yr[j] = from_f<T>(gt.k1 * ex2(fmaf(to_f(xr[j]) + gt.shift, gt.c, gt.off)));
+    // a vector whose two neighbours do not both lie inside the row (its first and last ones) is done element by element
+    const uintptr_t x_lo = reinterpret_cast<uintptr_t>(xr), x_hi = reinterpret_cast<uintptr_t>(xr + n);
+    for (int j0 = t; j0 < w.vecs; j0 += 2 * nt) {
+      Vec16 lo[2], hi[2];
+      bool inside[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = j0 + u * nt;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(xb + static_cast<int64_t>(j) * E) - s;
+        inside[u] = j < w.vecs && at >= x_lo && at + 32 <= x_hi;
+        if (inside[u]) {
+          lo[u] = ld_keep(reinterpret_cast<const void*>(at));
+          hi[u] = ld_keep(reinterpret_cast<const void*>(at + 16));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = j0 + u * nt;
+        if (j >= w.vecs) continue;
+        const int64_t c = static_cast<int64_t>(j) * E;
+        if (inside[u]) {
+          grad_vec<T>(shifted_vec(lo[u], hi[u], s), gt, yb + c);
+        } else {
+          for (int e = 0; e < E; ++e) grad_one(xb + c + e, yb + c + e, gt);
+        }
+      }
+    }
+  }
+  if (t < w.head + w.tail) {
+    const int64_t c = t < w.head ? t : n - w.tail + (t - w.head);
+    grad_one(xr + c, yr + c, gt);
   }
   // the label column, rewritten by the thread that wrote its vector or element
-  const int64_t unit = V > 1 ? col / V : col;
-  if (static_cast<int>(unit % nt) == t) yr[col] = from_f<T>(gt.k1 * expm1f(static_cast<float>(logp)));
+  if (col >= 0 && col < n) {
+    int64_t owner;
+    if (col < w.head) owner = col;
+    else if (col >= n - w.tail) owner = w.head + (col - (n - w.tail));
+    else owner = (col - w.head) / E % nt;
+    if (owner == t) yr[col] = from_f<T>(gt.k1 * expm1f(static_cast<float>(logp)));
+  }
 }
 
-template <typename T, int V> DSLPG_DEV void zero_row(T* yr, const LossRows& a, int t, int nt) {
-  if constexpr (V > 1) {
-    for (int j = t; j < a.nvec; j += nt) st_stream(yr + static_cast<int64_t>(j) * V, Vec16{{0u, 0u, 0u, 0u}});
-  } else {
-    for (int64_t j = t; j < a.N; j += nt) yr[j] = from_f<T>(0.f);
-  }
+template <typename T> DSLPG_DEV void zero_row(T* yr, int64_t n, int t, int nt) {
+  constexpr int E = Elt<T>::kPerVec;
+  const Stretch<T> w(yr, n);
+  for (int j = t; j < w.vecs; j += nt) st_stream(yr + w.head + static_cast<int64_t>(j) * E, Vec16{{0u, 0u, 0u, 0u}});
+  if (t < w.head + w.tail) yr[t < w.head ? t : n - w.tail + (t - w.head)] = from_f<T>(0.f);
 }
 
 // Beyond this a float32 lse no longer tells the row's probabilities to 2e-5 (a
 // row masked with the type's lowest value throughout has lse = -3e38 + ln N).
 constexpr float kLseTrusted = 256.f;
 
-// The gradient alone, from the forward's lse: a CTA a row, read once and written
-// once. Rows whose lse is beyond kLseTrusted have their statistics formed again.
-template <int KIND, typename T, int V>
-__global__ void __launch_bounds__(256) loss_bwd_kernel(const LossRows a, const PolicyTerms pol, const PairTerms pair,
-                                                       const GradOut o) {
+// The gradient alone, from the forward's lse: `tpr` threads a row, or (few long
+// rows) gridDim.y CTAs a row, each a stretch of its columns; read once and
+// written once. Rows whose lse is beyond kLseTrusted have their statistics formed
+// again.
+template <int KIND, typename T>
+__global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ LossRows a,
+                                                       const __grid_constant__ PolicyTerms pol,
+                                                       const __grid_constant__ PairTerms pair, const GradOut o) {
   __shared__ float red[2][32];
-  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
-    T* yr = static_cast<T*>(o.dx) + r * o.ldo;
-    const int64_t col = label_col(a, r);
-    int64_t seq = 0;
-    if (KIND == kPair && col >= 0) seq = sequence_of(pair, r, a.M);
-    if (col < 0 || seq < 0) {
-      zero_row<T, V>(yr, a, threadIdx.x, blockDim.x);
-      continue;
+  const int g0 = threadIdx.x / a.tpr, t = threadIdx.x - g0 * a.tpr;
+  const int nw = a.tpr >> 5, first_warp = g0 * nw;
+  const int64_t part = ((a.N + gridDim.y - 1) / gridDim.y + 63) & ~63ll, lo = part * blockIdx.y;
+  const int64_t n = lo + part < a.N ? part : a.N - lo;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.rpc; base < a.M; base += step) {
+    const int64_t r = base + g0;
+    int64_t col = -1, seq = 0;
+    if (r < a.M) {
+      col = label_col(a, r);
+      if (KIND == kPair && col >= 0 && (seq = sequence_of(pair, r, a.M)) < 0) col = -1;
     }
+    T* yr = static_cast<T*>(o.dx) + r * o.ldo + lo;
     const T* xr = static_cast<const T*>(a.x) + r * a.ld;
-    const float lse = o.lse[r], xl = to_f(xr[col]);
+    float lse = 0.f, xl = 0.f;
+    if (col >= 0) {
+      lse = o.lse[r];
+      xl = to_f(xr[col]);
+    }
     double logp = static_cast<double>(xl) * a.scale - static_cast<double>(lse);
     // p = 2^((x - lse / scale) c); at scale 0 the row is uniform
     GradTerms gt{0.f, 0.f, a.c_hi, -lse * kLog2e};
@@ -408,16 +532,23 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const LossRows a, const P
       gt.shift = -static_cast<float>(static_cast<double>(lse) / a.scale);
       gt.off = 0.f;
     }
-    if (!(fabsf(lse) <= kLseTrusted)) {
+    const bool again = !(fabsf(lse) <= kLseTrusted);
+    if (__syncthreads_or(again)) {  // the CTA's rows together: the reductions have barriers
       Stat st;
-      fold_row<T, V, 1>(st, xr, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
-      const int nw = blockDim.x >> 5;
-      const float gm = group_reduce<MaxOp>(st.m, red[0], nw, 0);
-      const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, 0);
-      const RowStat rs(gm, gs, a);
-      logp = rs.logp(a, xl);
-      gt.shift = -rs.m;
-      gt.off = -rs.log2s;
+      if (again) fold_row<T, 1>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
+      const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
+      if (again) {
+        const RowStat rs(gm, gs, a);
+        logp = rs.logp(a, xl);
+        gt.shift = -rs.m;
+        gt.off = -rs.log2s;
+      }
+    }
+    if (r >= a.M || n <= 0) continue;
+    if (col < 0) {
+      zero_row<T>(yr, n, t, a.tpr);
+      continue;
     }
     float g, dl;
     if constexpr (KIND == kPolicy) {
@@ -428,114 +559,209 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const LossRows a, const P
       dl = o.dloss[(seq < pair.pairs ? seq : seq - pair.pairs) * o.dloss_stride];
     }
     gt.k1 = -(dl * g) * a.scale_f;
-    grad_row<T, V, 4>(xr, yr, a, gt, logp, col, threadIdx.x, blockDim.x);
+    grad_row<T, 4>(xr + lo, yr, n, gt, logp, col - lo, t, a.tpr);
   }
+}
+
+// p = 2^((x - m) c - log2 s) of a row whose statistics are known, dl = its dloss.
+DSLPG_DEV GradTerms grad_terms(const RowStat& rs, const LossRows& a, float dl, float g) {
+  return GradTerms{-(dl * g) * a.scale_f, -rs.m, a.c_hi, -rs.log2s};
 }
 
 constexpr int kFusedThreads = 1024;
 
-// Loss and gradient in one kernel: a CTA a row; the second reading of the row comes from L2.
-template <typename T, int V>
-__global__ void __launch_bounds__(kFusedThreads, 1) policy_fused_kernel(const LossRows a, const PolicyTerms pol,
-                                                                        const LossOut o, const GradOut go) {
+// Loss and gradient in one kernel, any row: `tpr` threads a row, whose second
+// reading comes from L1 or L2.
+template <typename T>
+__global__ void __launch_bounds__(kFusedThreads, 1) policy_two_pass_kernel(const __grid_constant__ LossRows a,
+                                                                           const __grid_constant__ PolicyTerms pol,
+                                                                           const LossOut o, const GradOut go) {
   __shared__ float red[2][32];
-  const int t = threadIdx.x;
-  uint64_t pol_keep;
-  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol_keep));
-  for (int64_t r = blockIdx.x; r < a.M; r += gridDim.x) {
+  const int g = threadIdx.x / a.tpr, t = threadIdx.x - g * a.tpr;
+  const int nw = a.tpr >> 5, first_warp = g * nw;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc;
+  uint64_t keep;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.rpc; base < a.M; base += step) {
+    const int64_t r = base + g;
+    const int64_t col = r < a.M ? label_col(a, r) : -1;
     const T* xr = static_cast<const T*>(a.x) + r * a.ld;
     T* yr = static_cast<T*>(go.dx) + r * go.ldo;
-    const int64_t col = label_col(a, r);
+    Stat st;
+    float xl = 0.f, dl = 0.f;
+    if (col >= 0) {
+      xl = to_f(xr[col]);
+      dl = go.dloss[r * go.dloss_stride];
+      fold_row<T, 4>(st, xr, a.N, a, t, a.tpr, [&](const void* p) {
+        Vec16 v;
+        asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+                     : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
+                     : "l"(p), "l"(keep));
+        return v;
+      });
+    }
+    const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
+    const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
+    if (r >= a.M) continue;
+    if (t == 0) write_row<kPolicy>(a, pol, o, r, col >= 0, xl, gm, gs);
     if (col < 0) {
-      zero_row<T, V>(yr, a, t, kFusedThreads);
-      if (t == 0) o.loss[r] = o.logp[r] = o.lse[r] = o.kl[r] = 0.f;
+      zero_row<T>(yr, a.N, t, a.tpr);
       continue;
     }
-    const float xl = to_f(xr[col]), dl = go.dloss[r * go.dloss_stride];
-    Stat st;
-    fold_row<T, V, 4>(st, xr, a, t, kFusedThreads, [&](const void* p) {
-      Vec16 v;
-      asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
-                   : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
-                   : "l"(p), "l"(pol_keep));
-      return v;
-    });
-    const float gm = group_reduce<MaxOp>(st.m, red[0], kFusedThreads / 32, 0);
-    const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], kFusedThreads / 32, 0);
     const RowStat rs(gm, gs, a);
     const double logp = rs.logp(a, xl);
-    const PolicyRow p = policy_row(pol, r, logp);
-    if (t == 0) {
-      o.loss[r] = p.loss;
-      o.logp[r] = static_cast<float>(logp);
-      o.lse[r] = static_cast<float>(rs.lse(a));
-      o.kl[r] = p.kl;
-    }
-    // p = 2^((x - m) c - log2 s)
-    const GradTerms gt{-(dl * p.g) * a.scale_f, -rs.m, a.c_hi, -rs.log2s};
-    grad_row<T, V, 2>(xr, yr, a, gt, logp, col, t, kFusedThreads);
+    grad_row<T, 2>(xr, yr, a.N, grad_terms(rs, a, dl, policy_row(pol, r, logp).g), logp, col, t, a.tpr);
   }
+}
+
+// Loss and gradient of rows that the registers of their threads hold (NV vectors
+// a thread, 16-byte rows): read once, written once.
+template <typename T, int NV>
+__global__ void __launch_bounds__(512) policy_short_kernel(const __grid_constant__ LossRows a,
+                                                           const __grid_constant__ PolicyTerms pol, const LossOut o,
+                                                           const GradOut go) {
+  constexpr int E = Elt<T>::kPerVec;
+  __shared__ float red[2][32];
+  const int g = threadIdx.x / a.tpr, t = threadIdx.x - g * a.tpr;
+  const int nw = a.tpr >> 5, first_warp = g * nw;
+  const int vecs = static_cast<int>(a.N / E);
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * a.rpc + g;
+  const int64_t col = r < a.M ? label_col(a, r) : -1;
+  const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+  T* yr = static_cast<T*>(go.dx) + r * go.ldo;
+  Vec16 v[NV];
+  float xl = 0.f, dl = 0.f;
+  Stat st;
+  if (col >= 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      v[k] = Vec16{{0u, 0u, 0u, 0u}};
+      if (t + k * a.tpr < vecs) v[k] = ld_stream(xr + static_cast<int64_t>(t + k * a.tpr) * E);
+    }
+    xl = to_f(xr[col]);
+    dl = go.dloss[r * go.dloss_stride];
+    if (t + (NV - 1) * a.tpr < vecs) {
+      fold_rows<T, NV>(st, v, a);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (t + k * a.tpr < vecs) {
+          const Vec16 one[1] = {v[k]};
+          fold_rows<T, 1>(st, one, a);
+        }
+      }
+    }
+  }
+  const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
+  const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
+  if (r >= a.M) return;
+  if (t == 0) write_row<kPolicy>(a, pol, o, r, col >= 0, xl, gm, gs);
+  if (col < 0) {
+    zero_row<T>(yr, a.N, t, a.tpr);
+    return;
+  }
+  const RowStat rs(gm, gs, a);
+  const double logp = rs.logp(a, xl);
+  const GradTerms gt = grad_terms(rs, a, dl, policy_row(pol, r, logp).g);
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (t + k * a.tpr < vecs) grad_vec<T>(v[k], gt, yr + static_cast<int64_t>(t + k * a.tpr) * E);
+  if (static_cast<int>(col / E % a.tpr) == t) yr[col] = from_f<T>(gt.k1 * expm1f(static_cast<float>(logp)));
 }
 
 namespace {
 
-template <int KIND, typename T, int V>
+// Threads of a row: about 16 vectors each, a warp at least, `most` at most.
+template <typename T> void set_threads(LossRows& a, int64_t n, int most) {
+  const int64_t want = (n / Elt<T>::kPerVec + 15) / 16;
+  a.tpr = static_cast<int>(want >= most ? most : (want + 31) / 32 * 32);
+  if (a.tpr < 32) a.tpr = 32;
+  a.rpc = a.tpr >= 256 ? 1 : 256 / a.tpr;
+}
+
+int ctas_of(const LossRows& a) {  // a CTA for each of its rows: the hardware hands them out as SMs become free
+  const int64_t n = (a.M + a.rpc - 1) / a.rpc;
+  return static_cast<int>(n < 0x7fffffff ? n : 0x7fffffff);
+}
+
+constexpr int64_t kSplitBytes = 32 * 1024;  // a CTA's stretch of a split row, at least
+
+template <int KIND, typename T>
 cudaError_t launch_rows(LossRows a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o, cudaStream_t st) {
-  // about 16 vectors (or 64 scalars) a thread, at most 256 threads a row
-  const int64_t units = V > 1 ? (a.nvec + 15) / 16 : (a.N + 63) / 64;
-  a.tpr = static_cast<int>(units >= 256 ? 256 : (units + 31) / 32 * 32);
-  a.rpc = 256 / a.tpr;
-  const int block = a.tpr * a.rpc;
-  const void* fn = reinterpret_cast<const void*>(&loss_rows_kernel<KIND, T, V>);
-  const int grid = persistent_grid(fn, block, 0, (a.M + a.rpc - 1) / a.rpc);
-  loss_rows_kernel<KIND, T, V><<<grid, block, 0, st>>>(a, pol, pair, o);
+  // few long rows: a cluster of up to 8 CTAs each
+  const int64_t bytes = a.N * static_cast<int64_t>(sizeof(T));
+  int C = 1;
+  while (C < 8 && a.M * C * 2 <= sm_count() && bytes / (C * 2) >= kSplitBytes) C *= 2;
+  if (C > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(C);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(a.M * C));
+    cfg.blockDim = dim3(512);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, loss_split_kernel<KIND, T>, a, pol, pair, o);
+  }
+  set_threads<T>(a, a.N, 256);
+  loss_rows_kernel<KIND, T><<<ctas_of(a), a.tpr * a.rpc, 0, st>>>(a, pol, pair, o);
   return cudaGetLastError();
 }
 
-template <int KIND, typename T, int V>
-cudaError_t launch_bwd(const LossRows& a, const PolicyTerms& pol, const PairTerms& pair, const GradOut& o,
-                       cudaStream_t st) {
-  const void* fn = reinterpret_cast<const void*>(&loss_bwd_kernel<KIND, T, V>);
-  loss_bwd_kernel<KIND, T, V><<<persistent_grid(fn, 256, 0, a.M), 256, 0, st>>>(a, pol, pair, o);
+template <int KIND, typename T>
+cudaError_t launch_bwd(LossRows a, const PolicyTerms& pol, const PairTerms& pair, const GradOut& o, cudaStream_t st) {
+  const int64_t bytes = a.N * static_cast<int64_t>(sizeof(T));
+  int split = 1;
+  while (split < 32 && a.M * split * 2 <= sm_count() * 4 && bytes / (split * 2) >= kSplitBytes / 2) split *= 2;
+  set_threads<T>(a, (a.N + split - 1) / split, 256);
+  loss_bwd_kernel<KIND, T><<<dim3(ctas_of(a), split), a.tpr * a.rpc, 0, st>>>(a, pol, pair, o);
   return cudaGetLastError();
 }
 
-template <typename T, int V>
-cudaError_t launch_fused(const LossRows& a, const PolicyTerms& pol, const LossOut& o, const GradOut& go,
-                         cudaStream_t st) {
-  const int64_t cap = sm_count();  // rows in flight stay in L2
-  policy_fused_kernel<T, V><<<static_cast<int>(a.M < cap ? a.M : cap), kFusedThreads, 0, st>>>(a, pol, o, go);
+template <typename T, int NV>
+cudaError_t launch_short(LossRows a, const PolicyTerms& pol, const LossOut& o, const GradOut& go, cudaStream_t st) {
+  const int64_t want = (a.N / Elt<T>::kPerVec + NV - 1) / NV;
+  a.tpr = static_cast<int>((want + 31) / 32 * 32);
+  a.rpc = a.tpr >= 128 ? 1 : 128 / a.tpr;
+  policy_short_kernel<T, NV><<<ctas_of(a), a.tpr * a.rpc, 0, st>>>(a, pol, o, go);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_fused(LossRows a, const PolicyTerms& pol, const LossOut& o, const GradOut& go, cudaStream_t st) {
+  constexpr int E = Elt<T>::kPerVec;
+  const bool vec = kernel_path() != DSLPG_PATH_STREAM && aligned(a.x, 16) && aligned(go.dx, 16) && a.N % E == 0 &&
+                   a.ld % E == 0 && go.ldo % E == 0;
+  const int64_t vecs = a.N / E;
+  if (vec && vecs <= 2 * 128) return launch_short<T, 2>(a, pol, o, go, st);
+  if (vec && vecs <= 8 * 512) return launch_short<T, 8>(a, pol, o, go, st);
+  set_threads<T>(a, a.N, kFusedThreads);
+  const int64_t cap = sm_count() * static_cast<int64_t>(a.tpr >= 512 ? 1 : 4);  // rows in flight stay in L2
+  const int64_t ctas = ctas_of(a);
+  policy_two_pass_kernel<T><<<static_cast<int>(ctas < cap ? ctas : cap), a.tpr * a.rpc, 0, st>>>(a, pol, o, go);
   return cudaGetLastError();
 }
 
 enum Way { kFwd, kBwd, kFwdBwd };
 
-template <int KIND, typename T, int V>
-cudaError_t launch_way(Way way, LossRows a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o,
-                       const GradOut& go, cudaStream_t st) {
-  a.nvec = V > 1 ? static_cast<int>(a.N / V) : 0;
-  if (way == kFwd) return launch_rows<KIND, T, V>(a, pol, pair, o, st);
-  if (way == kBwd) return launch_bwd<KIND, T, V>(a, pol, pair, go, st);
-  if constexpr (KIND == kPolicy) return launch_fused<T, V>(a, pol, o, go, st);
-  return cudaErrorNotSupported;
-}
-
 template <int KIND, typename T>
-cudaError_t dispatch_vec(Way way, const LossRows& a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o,
-                         const GradOut& go, cudaStream_t st) {
-  constexpr int E = Elt<T>::kPerVec;
-  const bool vec = kernel_path() != DSLPG_PATH_STREAM && aligned(a.x, 16) && a.N % E == 0 && a.ld % E == 0 &&
-                   (way == kFwd || (aligned(go.dx, 16) && go.ldo % E == 0));
-  return vec ? launch_way<KIND, T, E>(way, a, pol, pair, o, go, st) : launch_way<KIND, T, 1>(way, a, pol, pair, o, go, st);
+cudaError_t launch_way(Way way, const LossRows& a, const PolicyTerms& pol, const PairTerms& pair, const LossOut& o,
+                       const GradOut& go, cudaStream_t st) {
+  if (way == kFwd) return launch_rows<KIND, T>(a, pol, pair, o, st);
+  if (way == kBwd) return launch_bwd<KIND, T>(a, pol, pair, go, st);
+  if constexpr (KIND == kPolicy) return launch_fused<T>(a, pol, o, go, st);
+  return cudaErrorNotSupported;
 }
 
 template <int KIND>
 cudaError_t dispatch(Way way, int dt, const LossRows& a, const PolicyTerms& pol, const PairTerms& pair,
                      const LossOut& o, const GradOut& go, cudaStream_t st) {
   switch (dt) {
-    case DSLPG_F32: return dispatch_vec<KIND, float>(way, a, pol, pair, o, go, st);
-    case DSLPG_F16: return dispatch_vec<KIND, __half>(way, a, pol, pair, o, go, st);
-    default: return dispatch_vec<KIND, __nv_bfloat16>(way, a, pol, pair, o, go, st);
+    case DSLPG_F32: return launch_way<KIND, float>(way, a, pol, pair, o, go, st);
+    case DSLPG_F16: return launch_way<KIND, __half>(way, a, pol, pair, o, go, st);
+    default: return launch_way<KIND, __nv_bfloat16>(way, a, pol, pair, o, go, st);
   }
 }
 
