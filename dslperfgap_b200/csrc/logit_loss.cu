@@ -120,8 +120,11 @@ template <int n> DSLPG_DEV void fold_values(Stat& st, const float (&x)[n], const
   }
 }
 
-// NV vectors of logits, all valid.
-template <typename T, int NV>
+// NV vectors of logits, all valid. POLY > 0 (fused kernels, whose statistics are
+// for single rows and bound by the exponentials): the constant's second part is
+// left out and every POLY-th pair of exponentials goes to the FMA pipe
+// (exp2_poly2); both are below 1e-6 in lse.
+template <typename T, int NV, int POLY>
 DSLPG_DEV void fold_rows(Stat& st, const Vec16 (&v)[NV], const LossRows& a) {
   constexpr int P = Elt<T>::kPerVec / 2;
   const float ext = (a.sign >= 0.f) ? RawExtreme<T, NV, false>::run(v) : RawExtreme<T, NV, true>::run(v);
@@ -134,9 +137,16 @@ DSLPG_DEV void fold_rows(Stat& st, const Vec16 (&v)[NV], const LossRows& a) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const f32x2 y = add2(unpack_pair<T>(v[k], p), neg);
-      float d0, d1;
-      upk2(fma2(y, lo, mul2(y, hi)), d0, d1);
-      acc[p & 1] = add2(acc[p & 1], pk2(ex2(d0), ex2(d1)));
+      const f32x2 d = POLY ? mul2(y, hi) : fma2(y, lo, mul2(y, hi));
+      f32x2 e;
+      if (POLY && (k * P + p) % (POLY ? POLY : 1) == POLY - 1) {
+        e = exp2_poly2(d);
+      } else {
+        float d0, d1;
+        upk2(d, d0, d1);
+        e = pk2(ex2(d0), ex2(d1));
+      }
+      acc[p & 1] = add2(acc[p & 1], e);
     }
   st.rebase(nm, a);
   st.s += hsum2(add2(acc[0], acc[1]));
@@ -163,13 +173,12 @@ struct PolicyRow {
   float loss, kl, g;  // g: dloss / dlogp
 };
 
-DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, int64_t r, double logp) {
-  const float adv = p.adv[r * p.adv_stride];
-  const float ratio = expf(static_cast<float>(logp - static_cast<double>(p.old_logp[r * p.old_stride])));
+DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, float old_logp, float adv, float ref, double logp) {
+  const float ratio = expf(static_cast<float>(logp - static_cast<double>(old_logp)));
   const float l1 = -ratio * adv, l2 = -fminf(fmaxf(ratio, p.lo), p.hi) * adv;
   PolicyRow o{max_nan(l1, l2), 0.f, l2 > l1 ? 0.f : l1};
   if (p.ref != nullptr) {
-    const float d = static_cast<float>(static_cast<double>(p.ref[r * p.ref_stride]) - logp);
+    const float d = static_cast<float>(static_cast<double>(ref) - logp);
     const float e = expm1f(d);
     // exp(d) - d - 1; its power series near 0, where the difference cancels (|d| < 1/4: the first term left out is
     // below 2e-8 of the sum)
@@ -182,6 +191,11 @@ DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, int64_t r, double logp) {
     }
   }
   return o;
+}
+
+DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, int64_t r, double logp) {
+  return policy_row(p, p.old_logp[r * p.old_stride], p.adv[r * p.adv_stride],
+                    p.ref != nullptr ? p.ref[r * p.ref_stride] : 0.f, logp);
 }
 
 // dloss g of a preference row in sequence `seq` (chosen ones first).
@@ -213,7 +227,7 @@ template <typename T> struct Stretch {
 // Fold elements [0, n) from xr on with `tpr` threads, this one being t: 16-byte
 // vectors, the next ones loaded before this round's arithmetic, and the elements
 // before the first and behind the last whole vector, one a thread.
-template <typename T, int U, class Load>
+template <typename T, int U, int POLY, class Load>
 DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int t, int tpr, Load ld) {
   constexpr int E = Elt<T>::kPerVec;
   const Stretch<T> w(xr, n);
@@ -240,13 +254,13 @@ DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int
     for (int u = 0; u < U; ++u) v[u] = nx[u];
     if (j0 + stride < w.vecs) load(nx, j0 + stride);
     if (j0 + (U - 1) * tpr < w.vecs) {
-      fold_rows<T, U>(st, v, a);
+      fold_rows<T, U, POLY>(st, v, a);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (j0 + u * tpr < w.vecs) {
           const Vec16 one[1] = {v[u]};
-          fold_rows<T, 1>(st, one, a);
+          fold_rows<T, 1, POLY>(st, one, a);
         }
       }
     }
@@ -298,7 +312,7 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
     float xl = 0.f;
     if (col >= 0) {
       if (t == 0) xl = to_f(xr[col]);
-      fold_row<T, 4>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      fold_row<T, 4, 0>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
     }
     const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
     const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
@@ -326,7 +340,7 @@ __global__ void __launch_bounds__(512) loss_split_kernel(const __grid_constant__
     const T* xr = static_cast<const T*>(a.x) + r * a.ld;
     const int64_t part = ((a.N + C - 1) / C + 63) & ~63ll, lo = part * rank, n = lo + part < a.N ? part : a.N - lo;
     if (threadIdx.x == 0 && rank == 0) xl = to_f(xr[col]);
-    if (n > 0) fold_row<T, 4>(st, xr + lo, n, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
+    if (n > 0) fold_row<T, 4, 0>(st, xr + lo, n, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
   }
   const float gm = rd.template reduce<MaxOp>(st.m);
   const float gs = rd.template reduce<SumOp>(merged(st, gm, a));
@@ -414,13 +428,14 @@ DSLPG_DEV Vec16 shifted_vec(const Vec16& lo, const Vec16& hi, int s) {
 // column (col, if in there): k1 expm1(logp). Vectors are those of the output; the
 // logits' may lie at another distance from a 16-byte boundary (rows of odd
 // length). The next chunk's loads are issued before this chunk's arithmetic.
-template <typename T, int U>
+// SAME: they lie at the same one in every row.
+template <typename T, int U, bool SAME>
 DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
   constexpr int E = Elt<T>::kPerVec;
   const Stretch<T> w(yr, n);
   const T* xb = xr + w.head;
   T* yb = yr + w.head;
-  const int s = static_cast<int>(reinterpret_cast<uintptr_t>(xb) & 15);
+  const int s = SAME ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xb) & 15);
   if (s == 0) {
     auto load = [&](Vec16 (&dst)[U], int j0) {
 #pragma unroll
@@ -443,7 +458,7 @@ DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, doub
         if (j < w.vecs) grad_vec<T>(v[u], gt, yb + static_cast<int64_t>(j) * E);
       }
     }
-  } else {
+  } else if constexpr (!SAME) {
     // a vector whose two neighbours do not both lie inside the row (its first and last ones) is done element by element
     const uintptr_t x_lo = reinterpret_cast<uintptr_t>(xr), x_hi = reinterpret_cast<uintptr_t>(xr + n);
     for (int j0 = t; j0 < w.vecs; j0 += 2 * nt) {
@@ -501,7 +516,7 @@ constexpr float kLseTrusted = 256.f;
 // rows) gridDim.y CTAs a row, each a stretch of its columns; read once and
 // written once. Rows whose lse is beyond kLseTrusted have their statistics formed
 // again.
-template <int KIND, typename T>
+template <int KIND, typename T, bool SAME>
 __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ LossRows a,
                                                        const __grid_constant__ PolicyTerms pol,
                                                        const __grid_constant__ PairTerms pair, const GradOut o) {
@@ -535,7 +550,7 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ L
     const bool again = !(fabsf(lse) <= kLseTrusted);
     if (__syncthreads_or(again)) {  // the CTA's rows together: the reductions have barriers
       Stat st;
-      if (again) fold_row<T, 1>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      if (again) fold_row<T, 1, 0>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
       const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
       const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
       if (again) {
@@ -559,7 +574,7 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ L
       dl = o.dloss[(seq < pair.pairs ? seq : seq - pair.pairs) * o.dloss_stride];
     }
     gt.k1 = -(dl * g) * a.scale_f;
-    grad_row<T, 4>(xr + lo, yr, n, gt, logp, col - lo, t, a.tpr);
+    grad_row<T, 4, SAME>(xr + lo, yr, n, gt, logp, col - lo, t, a.tpr);
   }
 }
 
@@ -568,49 +583,87 @@ DSLPG_DEV GradTerms grad_terms(const RowStat& rs, const LossRows& a, float dl, f
   return GradTerms{-(dl * g) * a.scale_f, -rs.m, a.c_hi, -rs.log2s};
 }
 
-constexpr int kFusedThreads = 1024;
-
-// Loss and gradient in one kernel, any row: `tpr` threads a row, whose second
-// reading comes from L1 or L2.
-template <typename T>
-__global__ void __launch_bounds__(kFusedThreads, 1) policy_two_pass_kernel(const __grid_constant__ LossRows a,
-                                                                           const __grid_constant__ PolicyTerms pol,
-                                                                           const LossOut o, const GradOut go) {
+// Loss and gradient in one kernel, any row: a CTA a row, whose second reading
+// comes from L2 (the rows in flight, one an SM, are a third of it; the first
+// reading marks its lines to stay). Rows are taken NT at a time: of the counted
+// ones among them, and of the left-out ones, CTA k does every G-th by their
+// number, so that none gets more of either kind than another.
+// Measured on bf16 [8192, 128256] with 1024 rows left out (floor 605 us): TWO_PASS.
+template <typename T, int NT, bool SAME>
+__global__ void __launch_bounds__(NT, 1) policy_two_pass_kernel(const __grid_constant__ LossRows a,
+                                                                const __grid_constant__ PolicyTerms pol,
+                                                                const LossOut o, const GradOut go) {
   __shared__ float red[2][32];
-  const int g = threadIdx.x / a.tpr, t = threadIdx.x - g * a.tpr;
-  const int nw = a.tpr >> 5, first_warp = g * nw;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc;
-  uint64_t keep;
-  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.rpc; base < a.M; base += step) {
-    const int64_t r = base + g;
-    const int64_t col = r < a.M ? label_col(a, r) : -1;
-    const T* xr = static_cast<const T*>(a.x) + r * a.ld;
-    T* yr = static_cast<T*>(go.dx) + r * go.ldo;
-    Stat st;
-    float xl = 0.f, dl = 0.f;
-    if (col >= 0) {
-      xl = to_f(xr[col]);
-      dl = go.dloss[r * go.dloss_stride];
-      fold_row<T, 4>(st, xr, a.N, a, t, a.tpr, [&](const void* p) {
+  __shared__ int in_warp[32];
+  __shared__ int list_row[2][NT], list_col[NT];
+  constexpr int nw = NT / 32;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int64_t G = gridDim.x;
+  int64_t seen[2] = {0, 0};  // left-out and counted rows before the present ones
+  for (int64_t base = 0; base < a.M; base += NT) {
+    const int64_t mine = base + t;
+    const int64_t label = mine < a.M ? label_col(a, mine) : -1;
+    const bool counted = label >= 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, counted);
+    if (lane == 0) in_warp[warp] = __popc(mask);
+    __syncthreads();
+    int before = lane < nw && lane < warp ? in_warp[lane] : 0, total = lane < nw ? in_warp[lane] : 0;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, k);
+      total += __shfl_xor_sync(0xffffffffu, total, k);
+    }
+    before += __popc(mask & ((1u << lane) - 1u));  // counted rows of this block before mine
+    const int rows = static_cast<int>(a.M - base < NT ? a.M - base : NT);
+    // the first of CTA k's numbers from seen[kind] on, and how many of the block's rows have one
+    int64_t first[2] = {0, 0};
+    int count[2] = {0, 0};
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const int64_t n = kind ? total : rows - total;
+      first[kind] = seen[kind] + (static_cast<int64_t>(blockIdx.x) + G - seen[kind] % G) % G;
+      const int64_t ahead = seen[kind] + n - first[kind];
+      count[kind] = ahead > 0 ? static_cast<int>((ahead + G - 1) / G) : 0;
+    }
+    if (mine < a.M) {
+      const int64_t number = counted ? seen[1] + before - first[1] : seen[0] + (t - before) - first[0];
+      if (number >= 0 && number % G == 0) {
+        list_row[counted][number / G] = t;
+        if (counted) list_col[number / G] = static_cast<int>(label);
+      }
+    }
+    __syncthreads();
+    seen[0] += rows - total;
+    seen[1] += total;
+    for (int n = 0; n < count[1]; ++n) {
+      const int64_t r = base + list_row[1][n];
+      const int col = list_col[n];
+      const T* xr = static_cast<const T*>(a.x) + r * a.ld;
+      const float xl = to_f(xr[col]), dl = go.dloss[r * go.dloss_stride];
+      uint64_t keep;
+      asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      Stat st;
+      fold_row<T, 4, 4>(st, xr, a.N, a, t, NT, [&](const void* p) {
         Vec16 v;
         asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                      : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
                      : "l"(p), "l"(keep));
         return v;
       });
+      const float gm = group_reduce<MaxOp>(st.m, red[0], nw, 0);
+      const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, 0);
+      if (t == 0) write_row<kPolicy>(a, pol, o, r, true, xl, gm, gs);
+      const RowStat rs(gm, gs, a);
+      const double logp = rs.logp(a, xl);
+      grad_row<T, 2, SAME>(xr, static_cast<T*>(go.dx) + r * go.ldo, a.N, grad_terms(rs, a, dl, policy_row(pol, r, logp).g),
+                     logp, col, t, NT);
     }
-    const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
-    const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
-    if (r >= a.M) continue;
-    if (t == 0) write_row<kPolicy>(a, pol, o, r, col >= 0, xl, gm, gs);
-    if (col < 0) {
-      zero_row<T>(yr, a.N, t, a.tpr);
-      continue;
+    for (int n = 0; n < count[0]; ++n) {
+      const int64_t r = base + list_row[0][n];
+      zero_row<T>(static_cast<T*>(go.dx) + r * go.ldo, a.N, t, NT);
+      if (t == 0) o.loss[r] = o.logp[r] = o.lse[r] = o.kl[r] = 0.f;
     }
-    const RowStat rs(gm, gs, a);
-    const double logp = rs.logp(a, xl);
-    grad_row<T, 2>(xr, yr, a.N, grad_terms(rs, a, dl, policy_row(pol, r, logp).g), logp, col, t, a.tpr);
+    __syncthreads();  // the lists are written again
   }
 }
 
@@ -641,13 +694,13 @@ __global__ void __launch_bounds__(512) policy_short_kernel(const __grid_constant
     xl = to_f(xr[col]);
     dl = go.dloss[r * go.dloss_stride];
     if (t + (NV - 1) * a.tpr < vecs) {
-      fold_rows<T, NV>(st, v, a);
+      fold_rows<T, NV, 4>(st, v, a);
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if (t + k * a.tpr < vecs) {
           const Vec16 one[1] = {v[k]};
-          fold_rows<T, 1>(st, one, a);
+          fold_rows<T, 1, 4>(st, one, a);
         }
       }
     }
@@ -684,6 +737,12 @@ int ctas_of(const LossRows& a) {  // a CTA for each of its rows: the hardware ha
   return static_cast<int>(n < 0x7fffffff ? n : 0x7fffffff);
 }
 
+// Whether a row's logits and its gradients lie at the same distance from a 16-byte boundary, in every row.
+template <typename T> bool same_phase(const LossRows& a, const GradOut& o) {
+  const uintptr_t apart = reinterpret_cast<uintptr_t>(a.x) - reinterpret_cast<uintptr_t>(o.dx);
+  return apart % 16 == 0 && (a.ld - o.ldo) * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+}
+
 constexpr int64_t kSplitBytes = 32 * 1024;  // a CTA's stretch of a split row, at least
 
 template <int KIND, typename T>
@@ -716,7 +775,9 @@ cudaError_t launch_bwd(LossRows a, const PolicyTerms& pol, const PairTerms& pair
   int split = 1;
   while (split < 32 && a.M * split * 2 <= sm_count() * 4 && bytes / (split * 2) >= kSplitBytes / 2) split *= 2;
   set_threads<T>(a, (a.N + split - 1) / split, 256);
-  loss_bwd_kernel<KIND, T><<<dim3(ctas_of(a), split), a.tpr * a.rpc, 0, st>>>(a, pol, pair, o);
+  const dim3 grid(ctas_of(a), split);
+  if (same_phase<T>(a, o)) loss_bwd_kernel<KIND, T, true><<<grid, a.tpr * a.rpc, 0, st>>>(a, pol, pair, o);
+  else loss_bwd_kernel<KIND, T, false><<<grid, a.tpr * a.rpc, 0, st>>>(a, pol, pair, o);
   return cudaGetLastError();
 }
 
@@ -737,10 +798,15 @@ cudaError_t launch_fused(LossRows a, const PolicyTerms& pol, const LossOut& o, c
   const int64_t vecs = a.N / E;
   if (vec && vecs <= 2 * 128) return launch_short<T, 2>(a, pol, o, go, st);
   if (vec && vecs <= 8 * 512) return launch_short<T, 8>(a, pol, o, go, st);
-  set_threads<T>(a, a.N, kFusedThreads);
-  const int64_t cap = sm_count() * static_cast<int64_t>(a.tpr >= 512 ? 1 : 4);  // rows in flight stay in L2
-  const int64_t ctas = ctas_of(a);
-  policy_two_pass_kernel<T><<<static_cast<int>(ctas < cap ? ctas : cap), a.tpr * a.rpc, 0, st>>>(a, pol, o, go);
+  // rows in flight stay in L2: one CTA of 1024 threads an SM, or several small ones
+  const int64_t most = vecs > 4 * 256 ? sm_count() : 8 * sm_count();
+  const int grid = static_cast<int>(a.M < most ? a.M : most);
+  auto launch = [&](auto small, auto large) {
+    if (vecs > 4 * 256) large<<<grid, 1024, 0, st>>>(a, pol, o, go);
+    else small<<<grid, 128, 0, st>>>(a, pol, o, go);
+  };
+  if (same_phase<T>(a, go)) launch(&policy_two_pass_kernel<T, 128, true>, &policy_two_pass_kernel<T, 1024, true>);
+  else launch(&policy_two_pass_kernel<T, 128, false>, &policy_two_pass_kernel<T, 1024, false>);
   return cudaGetLastError();
 }
 
@@ -827,6 +893,7 @@ int pair_args(PairTerms& p, const dslpg_pair_terms* h, int64_t rows, bool fwd) {
 }
 
 }  // namespace
+
 }  // namespace dslpg
 
 using namespace dslpg;
