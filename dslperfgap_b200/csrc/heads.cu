@@ -79,7 +79,7 @@ enum HeadOp : int { kRotate, kNorm, kNormBwd };
 // V elements of T.
 template <typename T, int V> struct Pack {
   static constexpr int kBytes = V * static_cast<int>(sizeof(T));
-  static_assert(kBytes == 8 || kBytes == 16, "8- or 16-byte vectors");
+  static_assert(kBytes == 4 || kBytes == 8 || kBytes == 16, "4-, 8- or 16-byte vectors");
 };
 
 // Plain float32 arithmetic throughout: packed pairs (fma.f32x2) took more
@@ -88,6 +88,7 @@ template <typename T, int V> struct Pack {
 template <typename T, int V> DSLPG_DEV void lds_vec(uint32_t at, float (&f)[V]) {
   Vec16 v{{0u, 0u, 0u, 0u}};
   if constexpr (Pack<T, V>::kBytes == 16) v = lds16(at);
+  else if constexpr (Pack<T, V>::kBytes == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v.w[0]) : "r"(at) : "memory");
   else asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.w[0]), "=r"(v.w[1]) : "r"(at) : "memory");
   float all[Elt<T>::kPerVec];
   unpack<T>(v, all);
@@ -97,6 +98,7 @@ template <typename T, int V> DSLPG_DEV void lds_vec(uint32_t at, float (&f)[V]) 
 
 template <typename T, int V> DSLPG_DEV void st_vec(T* dst, const float (&f)[V]) {
   if constexpr (sizeof(T) == 4 && V == 2) st_stream8(dst, __float_as_uint(f[0]), __float_as_uint(f[1]));
+  else if constexpr (V == 2) asm volatile("st.global.u32 [%0], %1;" ::"l"(dst), "r"(pack2<T>(f[0], f[1])) : "memory");
   else StoreOut<T, V>::run(dst, f);
 }
 
@@ -896,6 +898,10 @@ cudaError_t dispatch(HeadArgs a, bool norm, bool bwd, float* dwq, float* dwk, cu
     if (fits<T>(a, E / 2))
       return a.interleaved ? launch_v<T, E / 2, true>(a, norm, bwd, dwq, dwk, st)
                            : launch_v<T, E / 2, false>(a, norm, bwd, dwq, dwk, st);
+    if constexpr (E > 4)
+      if (fits<T>(a, 2))  // pairs in fours but not in eights (36 of 72 features)
+        return a.interleaved ? launch_v<T, 2, true>(a, norm, bwd, dwq, dwk, st)
+                             : launch_v<T, 2, false>(a, norm, bwd, dwq, dwk, st);
   }
   if (bwd) return launch_any<T, true, true>(a, dwq, dwk, st);
   return norm ? launch_any<T, true, false>(a, dwq, dwk, st) : launch_any<T, false, false>(a, dwq, dwk, st);

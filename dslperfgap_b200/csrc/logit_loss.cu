@@ -16,14 +16,15 @@
 // preferences, when it lies in no sequence): its logits are not read, its
 // results and gradients are 0.
 //
-// Statistics: d = (x - m) scale log2(e) against the running extreme m (the
-// largest x, or the smallest for a negative scale), an online sum of 2^d per
-// thread; then logp = scale (x_y - m) - ln s and lse = scale m + ln s, in 64 bits
-// once per row. x - m is 0 at the extreme whatever its size, so a row masked
-// with the type's lowest value throughout is a uniform row. The constant has two
-// float32 parts: rounded to one it would shift every lse of a call in the same
-// direction (some 2e-7), which a sum over a sequence's rows adds up. Both parts
-// have one sign, so that a logit of -inf gives d = -inf and not NaN.
+// Statistics: with c = scale log2(e) and m the running extreme (the largest x, or
+// the smallest for a negative scale), an online sum of 2^(x c - R) per thread,
+// R = m c as rounded; x c - R is one fma. What R lost is put back at the end,
+// in 64 bits once per row: logp = scale (x_y - m) - ln s, lse = scale m + ln s.
+// Where |R| is 2^23 or more (a row masked with the type's lowest value
+// throughout), 2^((x - m) c) is summed instead, which is right for any size. c has
+// two float32 parts: rounded to one it would shift every lse of a call in the
+// same direction (some 5e-7), which a sum over a sequence's rows adds up. Both
+// parts have one sign, so that a logit of -inf gives -inf and not NaN.
 #include "common.cuh"
 #include "pipe.cuh"
 
@@ -95,77 +96,102 @@ DSLPG_DEV int64_t sequence_of(const PairTerms& p, int64_t r, int64_t rows) {
   return lo;
 }
 
-// Online statistics of one thread: m = the largest sign * x, s = the sum of
-// 2^((sign x - m) |c|).
+constexpr float kPlainR = 8388608.f;  // 2^23
+
+// log2 of what a sum against the extreme m0 is multiplied with to be one against
+// m1 >= m0 (extremes as sign * x, ca = |c|).
+DSLPG_DEV float rebase_log2(float m0, float m1, float ca) {
+  const float r0 = m0 * ca, r1 = m1 * ca;
+  return fmaxf(fabsf(r0), fabsf(r1)) < kPlainR ? r0 - r1 : (m0 - m1) * ca;
+}
+
+// Online statistics of one thread: m = the largest sign * x, s the sum.
 struct Stat {
   float m = kNegInf, s = 0.f;
   DSLPG_DEV void rebase(float nm, const LossRows& a) {
-    if (m != nm && m != kNegInf) s *= ex2((m - nm) * fabsf(a.c_hi));  // s is 0 while m = -inf
+    if (m != nm && m != kNegInf) s *= ex2(rebase_log2(m, nm, fabsf(a.c_hi)));  // s is 0 while m = -inf
     m = nm;
   }
 };
 
-// n logits, of which those with ok[i] count.
-template <int n> DSLPG_DEV void fold_values(Stat& st, const float (&x)[n], const bool (&ok)[n], const LossRows& a) {
-  float nm = st.m;
-#pragma unroll
-  for (int i = 0; i < n; ++i)
-    if (ok[i]) nm = max_nan(nm, x[i] * a.sign);
+// One logit.
+DSLPG_DEV void fold_value(Stat& st, float x, const LossRows& a) {
+  const float nm = max_nan(st.m, x * a.sign);
   if (nm == kNegInf) return;  // nothing but -inf so far
   st.rebase(nm, a);
-#pragma unroll
-  for (int i = 0; i < n; ++i) {
-    const float y = x[i] - nm * a.sign;
-    if (ok[i]) st.s += ex2(fmaf(y, a.c_lo, y * a.c_hi));
-  }
+  const float r = nm * fabsf(a.c_hi);
+  const float y = fabsf(r) < kPlainR ? x : x - nm * a.sign;
+  st.s += ex2(fmaf(y, a.c_lo, fmaf(y, a.c_hi, fabsf(r) < kPlainR ? -r : 0.f)));
 }
 
-// NV vectors of logits, all valid. POLY > 0 (fused kernels, whose statistics are
-// for single rows and bound by the exponentials): the constant's second part is
-// left out and every POLY-th pair of exponentials goes to the FMA pipe
-// (exp2_poly2); both are below 1e-6 in lse.
-template <typename T, int NV, int POLY>
+// NV vectors of logits, all valid. PACKED: two to an instruction (fma.f32x2),
+// which the forward kernel gains by (201 us against 208 for the batch below, at
+// 3 CTAs an SM); the fused one, at 64 registers a thread, spills with it.
+template <typename T, int NV, bool PACKED>
 DSLPG_DEV void fold_rows(Stat& st, const Vec16 (&v)[NV], const LossRows& a) {
-  constexpr int P = Elt<T>::kPerVec / 2;
+  constexpr int E = Elt<T>::kPerVec;
   const float ext = (a.sign >= 0.f) ? RawExtreme<T, NV, false>::run(v) : RawExtreme<T, NV, true>::run(v);
   const float nm = max_nan(st.m, ext * a.sign);
   if (nm == kNegInf) return;
-  const f32x2 hi = pk2(a.c_hi, a.c_hi), lo = pk2(a.c_lo, a.c_lo), neg = pk2(-nm * a.sign, -nm * a.sign);
-  f32x2 acc[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+  const float r = nm * fabsf(a.c_hi), m = nm * a.sign;
+  float acc[2] = {0.f, 0.f};
+  if (!(fabsf(r) < kPlainR)) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      float x[E];
+      unpack<T>(v[k], x);
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const f32x2 y = add2(unpack_pair<T>(v[k], p), neg);
-      const f32x2 d = POLY ? mul2(y, hi) : fma2(y, lo, mul2(y, hi));
-      f32x2 e;
-      if (POLY && (k * P + p) % (POLY ? POLY : 1) == POLY - 1) {
-        e = exp2_poly2(d);
-      } else {
-        float d0, d1;
-        upk2(d, d0, d1);
-        e = pk2(ex2(d0), ex2(d1));
-      }
-      acc[p & 1] = add2(acc[p & 1], e);
+      for (int e = 0; e < E; ++e) acc[e & 1] += ex2(fmaf(x[e] - m, a.c_lo, (x[e] - m) * a.c_hi));
     }
+  } else if constexpr (PACKED) {
+    const f32x2 hi = pk2(a.c_hi, a.c_hi), lo = pk2(a.c_lo, a.c_lo), neg = pk2(-r, -r);
+    f32x2 sum[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int p = 0; p < E / 2; ++p) {
+        const f32x2 x = unpack_pair<T>(v[k], p);
+        float d0, d1;
+        upk2(fma2(x, lo, fma2(x, hi, neg)), d0, d1);
+        sum[p & 1] = add2(sum[p & 1], pk2(ex2(d0), ex2(d1)));
+      }
+    acc[0] = hsum2(add2(sum[0], sum[1]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float x[E];
+      unpack<T>(v[k], x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e & 1] += ex2(fmaf(x[e], a.c_lo, fmaf(x[e], a.c_hi, -r)));
+    }
+  }
   st.rebase(nm, a);
-  st.s += hsum2(add2(acc[0], acc[1]));
+  st.s += acc[0] + acc[1];
 }
 
 // A thread's sum against the row's extreme.
 DSLPG_DEV float merged(const Stat& st, float gm, const LossRows& a) {
-  return (st.m == gm || st.m == kNegInf) ? st.s : st.s * ex2((st.m - gm) * fabsf(a.c_hi));
+  return (st.m == gm || st.m == kNegInf) ? st.s : st.s * ex2(rebase_log2(st.m, gm, fabsf(a.c_hi)));
 }
 
 // A row's merged statistics. Where the extreme is not finite, all of it is NaN.
 struct RowStat {
-  float m, log2s;  // the extreme x itself; log2 of the sum
-  DSLPG_DEV RowStat(float gm, float gs, const LossRows& a)
-      : m(gm * a.sign), log2s(fabsf(gm) < kPosInf ? log2f(gs) : __builtin_nanf("")) {}
-  DSLPG_DEV double ln_s() const { return 0.69314718055994530942 * static_cast<double>(log2s); }
+  float m, r;     // the extreme x itself; m c as rounded
+  float log2_sum;  // of the sum as it was formed
+  double log2_s;  // of the sum of 2^((x - m) c)
+  DSLPG_DEV RowStat(float gm, float gs, const LossRows& a) : m(gm * a.sign), r(gm * fabsf(a.c_hi)) {
+    log2_sum = fabsf(gm) < kPosInf ? log2f(gs) : __builtin_nanf("");
+    log2_s = log2_sum;
+    if (fabsf(r) < kPlainR) {
+      const double c = static_cast<double>(a.c_hi) + static_cast<double>(a.c_lo);
+      log2_s += static_cast<double>(r) - static_cast<double>(m) * c;
+    }
+  }
+  DSLPG_DEV double ln_s() const { return 0.69314718055994530942 * log2_s; }
   DSLPG_DEV double lse(const LossRows& a) const { return a.scale * static_cast<double>(m) + ln_s(); }
   DSLPG_DEV double logp(const LossRows& a, float xl) const {
-    return a.scale * (static_cast<double>(xl) - static_cast<double>(m)) - ln_s();
+    const double v = a.scale * (static_cast<double>(xl) - static_cast<double>(m)) - ln_s();
+    return v > 0.0 ? 0.0 : v;  // rounding may leave the only column with a probability 1e-8 above 0
   }
 };
 
@@ -227,7 +253,7 @@ template <typename T> struct Stretch {
 // Fold elements [0, n) from xr on with `tpr` threads, this one being t: 16-byte
 // vectors, the next ones loaded before this round's arithmetic, and the elements
 // before the first and behind the last whole vector, one a thread.
-template <typename T, int U, int POLY, class Load>
+template <typename T, int U, bool PACKED, class Load>
 DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int t, int tpr, Load ld) {
   constexpr int E = Elt<T>::kPerVec;
   const Stretch<T> w(xr, n);
@@ -244,9 +270,7 @@ DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int
   Vec16 nx[U];
   load(nx, t);
   if (t < w.head + w.tail) {
-    const float x[1] = {to_f(t < w.head ? xr[t] : xr[n - w.tail + (t - w.head)])};
-    const bool ok[1] = {true};
-    fold_values<1>(st, x, ok, a);
+    fold_value(st, to_f(t < w.head ? xr[t] : xr[n - w.tail + (t - w.head)]), a);
   }
   for (int j0 = t; j0 < w.vecs; j0 += stride) {
     Vec16 v[U];
@@ -254,13 +278,13 @@ DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int
     for (int u = 0; u < U; ++u) v[u] = nx[u];
     if (j0 + stride < w.vecs) load(nx, j0 + stride);
     if (j0 + (U - 1) * tpr < w.vecs) {
-      fold_rows<T, U, POLY>(st, v, a);
+      fold_rows<T, U, PACKED>(st, v, a);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (j0 + u * tpr < w.vecs) {
           const Vec16 one[1] = {v[u]};
-          fold_rows<T, 1, POLY>(st, one, a);
+          fold_rows<T, 1, PACKED>(st, one, a);
         }
       }
     }
@@ -270,11 +294,10 @@ DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int
 // The results of a row that counts, or of one that is left out.
 template <int KIND>
 DSLPG_DEV void write_row(const LossRows& a, const PolicyTerms& pol, const LossOut& o, int64_t r, bool counts, float xl,
-                         float gm, float gs) {
+                         const RowStat& rs) {
   double logp = 0.0, lse = 0.0;
   PolicyRow p{0.f, 0.f, 0.f};
   if (counts) {
-    const RowStat rs(gm, gs, a);
     lse = rs.lse(a);
     logp = rs.logp(a, xl);
     if constexpr (KIND == kPolicy) p = policy_row(pol, r, logp);
@@ -294,10 +317,14 @@ template <int KIND> DSLPG_DEV int64_t counted_col(const LossRows& a, const PairT
   return col;
 }
 
-// Row statistics: `tpr` threads a row. Writes the row's losses (policy) or its
+// Row statistics: `tpr` threads a row. HBM-bound: bf16 [6000, 128256] with 1500
+// rows left out takes 188 us (6.14 TB/s of 6.51 measured) with 4 loads in flight a
+// thread and 4 CTAs an SM; 3 CTAs 202, 5 193; 2, 3, 6 and 8 loads 197, 194, 223, 221.
+// A CTA a row, handed out by the hardware: shared out evenly beforehand, rows that
+// are left out leave some CTAs with less than others (261 us). Writes the row's losses (policy) or its
 // logp and lse (preferences; pair_kernel then sums them).
 template <int KIND, typename T>
-__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant__ LossRows a,
+__global__ void __launch_bounds__(256, 4) loss_rows_kernel(const __grid_constant__ LossRows a,
                                                            const __grid_constant__ PolicyTerms pol,
                                                            const __grid_constant__ PairTerms pair, const LossOut o) {
   __shared__ float red[2][32];
@@ -312,11 +339,11 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
     float xl = 0.f;
     if (col >= 0) {
       if (t == 0) xl = to_f(xr[col]);
-      fold_row<T, 4, 0>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      fold_row<T, 4, true>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
     }
     const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
     const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
-    if (t == 0 && r < a.M) write_row<KIND>(a, pol, o, r, col >= 0, xl, gm, gs);
+    if (t == 0 && r < a.M) write_row<KIND>(a, pol, o, r, col >= 0, xl, RowStat(gm, gs, a));
   }
 }
 
@@ -340,11 +367,11 @@ __global__ void __launch_bounds__(512) loss_split_kernel(const __grid_constant__
     const T* xr = static_cast<const T*>(a.x) + r * a.ld;
     const int64_t part = ((a.N + C - 1) / C + 63) & ~63ll, lo = part * rank, n = lo + part < a.N ? part : a.N - lo;
     if (threadIdx.x == 0 && rank == 0) xl = to_f(xr[col]);
-    if (n > 0) fold_row<T, 4, 0>(st, xr + lo, n, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
+    if (n > 0) fold_row<T, 4, true>(st, xr + lo, n, a, threadIdx.x, blockDim.x, [](const void* p) { return ld_stream(p); });
   }
   const float gm = rd.template reduce<MaxOp>(st.m);
   const float gs = rd.template reduce<SumOp>(merged(st, gm, a));
-  if (rank == 0 && threadIdx.x == 0) write_row<KIND>(a, pol, o, r, col >= 0, xl, gm, gs);
+  if (rank == 0 && threadIdx.x == 0) write_row<KIND>(a, pol, o, r, col >= 0, xl, RowStat(gm, gs, a));
   cl.sync();  // no CTA leaves while another may still read its slots
 }
 
@@ -383,27 +410,25 @@ __global__ void __launch_bounds__(256) pair_kernel(const LossRows a, const PairT
   }
 }
 
-// dlogits[c] = k1 2^((x + shift) c + off), with k1 = -dloss g scale.
+// dlogits[c] = k1 p with k1 = -dloss g scale; p = 2^(x c + off), or 2^((x + shift) c + off) where `far`: where off
+// would be so large (beyond kNear) that its rounding shows.
 struct GradTerms {
-  float k1, shift, c, off;
+  float k1, c, off, shift;
+  bool far;
 };
+constexpr float kNear = 64.f;
 
-// p = 2^((x + shift) c + off) times k1 for the elements of a vector.
-template <typename T> DSLPG_DEV void grad_vec(const Vec16& v, const GradTerms& gt, T* dst) {
-  constexpr int P = Elt<T>::kPerVec / 2;
-  const f32x2 c2 = pk2(gt.c, gt.c), sh2 = pk2(gt.shift, gt.shift), off2 = pk2(gt.off, gt.off), k2 = pk2(gt.k1, gt.k1);
-  f32x2 y[P];
+template <typename T, bool FAR> DSLPG_DEV void grad_vec(const Vec16& v, const GradTerms& gt, T* dst) {
+  constexpr int E = Elt<T>::kPerVec;
+  float x[E];
+  unpack<T>(v, x);
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    float d0, d1;
-    upk2(fma2(add2(unpack_pair<T>(v, p), sh2), c2, off2), d0, d1);
-    y[p] = mul2(k2, pk2(ex2(d0), ex2(d1)));
-  }
-  StorePairs<T, P>::run(dst, y);
+  for (int e = 0; e < E; ++e) x[e] = gt.k1 * ex2(fmaf(FAR ? x[e] + gt.shift : x[e], gt.c, gt.off));
+  StoreOut<T, E>::run(dst, x);
 }
 
 template <typename T> DSLPG_DEV void grad_one(const T* x, T* y, const GradTerms& gt) {
-  *y = from_f<T>(gt.k1 * ex2(fmaf(to_f(*x) + gt.shift, gt.c, gt.off)));
+  *y = from_f<T>(gt.k1 * ex2(fmaf(gt.far ? to_f(*x) + gt.shift : to_f(*x), gt.c, gt.off)));
 }
 
 // 16 bytes from any element on: the two vectors around them, shifted together.
@@ -429,8 +454,8 @@ DSLPG_DEV Vec16 shifted_vec(const Vec16& lo, const Vec16& hi, int s) {
 // logits' may lie at another distance from a 16-byte boundary (rows of odd
 // length). The next chunk's loads are issued before this chunk's arithmetic.
 // SAME: they lie at the same one in every row.
-template <typename T, int U, bool SAME>
-DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
+template <typename T, int U, bool SAME, bool FAR>
+DSLPG_DEV void grad_row_as(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
   constexpr int E = Elt<T>::kPerVec;
   const Stretch<T> w(yr, n);
   const T* xb = xr + w.head;
@@ -455,7 +480,7 @@ DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, doub
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * nt;
-        if (j < w.vecs) grad_vec<T>(v[u], gt, yb + static_cast<int64_t>(j) * E);
+        if (j < w.vecs) grad_vec<T, FAR>(v[u], gt, yb + static_cast<int64_t>(j) * E);
       }
     }
   } else if constexpr (!SAME) {
@@ -480,7 +505,7 @@ DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, doub
         if (j >= w.vecs) continue;
         const int64_t c = static_cast<int64_t>(j) * E;
         if (inside[u]) {
-          grad_vec<T>(shifted_vec(lo[u], hi[u], s), gt, yb + c);
+          grad_vec<T, FAR>(shifted_vec(lo[u], hi[u], s), gt, yb + c);
         } else {
           for (int e = 0; e < E; ++e) grad_one(xb + c + e, yb + c + e, gt);
         }
@@ -501,11 +526,24 @@ DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, doub
   }
 }
 
+template <typename T, int U, bool SAME>
+DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
+  if (gt.far) grad_row_as<T, 1, SAME, true>(xr, yr, n, gt, logp, col, t, nt);
+  else grad_row_as<T, U, SAME, false>(xr, yr, n, gt, logp, col, t, nt);
+}
+
 template <typename T> DSLPG_DEV void zero_row(T* yr, int64_t n, int t, int nt) {
   constexpr int E = Elt<T>::kPerVec;
   const Stretch<T> w(yr, n);
   for (int j = t; j < w.vecs; j += nt) st_stream(yr + w.head + static_cast<int64_t>(j) * E, Vec16{{0u, 0u, 0u, 0u}});
   if (t < w.head + w.tail) yr[t < w.head ? t : n - w.tail + (t - w.head)] = from_f<T>(0.f);
+}
+
+// Of a row whose statistics are known, dl = its dloss: p = 2^(x c - (R + log2 sum)), or 2^((x - m) c - log2 s).
+DSLPG_DEV GradTerms grad_terms(const RowStat& rs, const LossRows& a, float dl, float g) {
+  const float k1 = -(dl * g) * a.scale_f, off = rs.r + rs.log2_sum;
+  const bool far = !(fabsf(off) <= kNear && fabsf(rs.r) <= kNear);
+  return GradTerms{k1, a.c_hi, far ? -static_cast<float>(rs.log2_s) : -off, -rs.m, far};
 }
 
 // Beyond this a float32 lse no longer tells the row's probabilities to 2e-5 (a
@@ -514,7 +552,8 @@ constexpr float kLseTrusted = 256.f;
 
 // The gradient alone, from the forward's lse: `tpr` threads a row, or (few long
 // rows) gridDim.y CTAs a row, each a stretch of its columns; read once and
-// written once. Rows whose lse is beyond kLseTrusted have their statistics formed
+// written once. HBM-bound: 158 us for bf16 [2100, 128256] with 552 rows left out
+// (5.93 TB/s). Rows whose lse is beyond kLseTrusted have their statistics formed
 // again.
 template <int KIND, typename T, bool SAME>
 __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ LossRows a,
@@ -541,23 +580,23 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ L
       xl = to_f(xr[col]);
     }
     double logp = static_cast<double>(xl) * a.scale - static_cast<double>(lse);
-    // p = 2^((x - lse / scale) c); at scale 0 the row is uniform
-    GradTerms gt{0.f, 0.f, a.c_hi, -lse * kLog2e};
-    if (a.scale != 0.0) {
+    // p = 2^(x c - lse log2(e)), or 2^((x - lse / scale) c) (at scale 0 the row is uniform)
+    const double off = -1.4426950408889634074 * static_cast<double>(lse);
+    GradTerms gt{0.f, a.c_hi, static_cast<float>(off), 0.f, fabs(off) > static_cast<double>(kNear) && a.scale != 0.0};
+    if (gt.far) {
       gt.shift = -static_cast<float>(static_cast<double>(lse) / a.scale);
       gt.off = 0.f;
     }
     const bool again = !(fabsf(lse) <= kLseTrusted);
     if (__syncthreads_or(again)) {  // the CTA's rows together: the reductions have barriers
       Stat st;
-      if (again) fold_row<T, 1, 0>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
+      if (again) fold_row<T, 1, true>(st, xr, a.N, a, t, a.tpr, [](const void* p) { return ld_stream(p); });
       const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
       const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
       if (again) {
         const RowStat rs(gm, gs, a);
         logp = rs.logp(a, xl);
-        gt.shift = -rs.m;
-        gt.off = -rs.log2s;
+        gt = grad_terms(rs, a, 0.f, 0.f);
       }
     }
     if (r >= a.M || n <= 0) continue;
@@ -578,17 +617,18 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ L
   }
 }
 
-// p = 2^((x - m) c - log2 s) of a row whose statistics are known, dl = its dloss.
-DSLPG_DEV GradTerms grad_terms(const RowStat& rs, const LossRows& a, float dl, float g) {
-  return GradTerms{-(dl * g) * a.scale_f, -rs.m, a.c_hi, -rs.log2s};
-}
-
 // Loss and gradient in one kernel, any row: a CTA a row, whose second reading
 // comes from L2 (the rows in flight, one an SM, are a third of it; the first
 // reading marks its lines to stay). Rows are taken NT at a time: of the counted
 // ones among them, and of the left-out ones, CTA k does every G-th by their
 // number, so that none gets more of either kind than another.
-// Measured on bf16 [8192, 128256] with 1024 rows left out (floor 605 us): TWO_PASS.
+// Bound by instructions and latency: one pass of a row at a time is on an SM, so its
+// reading of HBM and its writing take turns. bf16 [8192, 128256] with 1024 rows left
+// out takes 812 us (floor 605); 768 threads 835, two CTAs of 512 827, a quarter of
+// the exponentials on the FMA pipe 817. A row kept in the shared memory of a
+// cluster (bulk copies, one read) was slower, 868 us: the ring holds 1.6 such rows
+// an SM, too little to cover the loads, the exchange of statistics and the gradient
+// behind one another.
 template <typename T, int NT, bool SAME>
 __global__ void __launch_bounds__(NT, 1) policy_two_pass_kernel(const __grid_constant__ LossRows a,
                                                                 const __grid_constant__ PolicyTerms pol,
@@ -643,7 +683,7 @@ __global__ void __launch_bounds__(NT, 1) policy_two_pass_kernel(const __grid_con
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
       Stat st;
-      fold_row<T, 4, 4>(st, xr, a.N, a, t, NT, [&](const void* p) {
+      fold_row<T, 4, false>(st, xr, a.N, a, t, NT, [&](const void* p) {
         Vec16 v;
         asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                      : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
@@ -652,8 +692,8 @@ __global__ void __launch_bounds__(NT, 1) policy_two_pass_kernel(const __grid_con
       });
       const float gm = group_reduce<MaxOp>(st.m, red[0], nw, 0);
       const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, 0);
-      if (t == 0) write_row<kPolicy>(a, pol, o, r, true, xl, gm, gs);
       const RowStat rs(gm, gs, a);
+      if (t == 0) write_row<kPolicy>(a, pol, o, r, true, xl, rs);
       const double logp = rs.logp(a, xl);
       grad_row<T, 2, SAME>(xr, static_cast<T*>(go.dx) + r * go.ldo, a.N, grad_terms(rs, a, dl, policy_row(pol, r, logp).g),
                      logp, col, t, NT);
@@ -694,13 +734,13 @@ __global__ void __launch_bounds__(512) policy_short_kernel(const __grid_constant
     xl = to_f(xr[col]);
     dl = go.dloss[r * go.dloss_stride];
     if (t + (NV - 1) * a.tpr < vecs) {
-      fold_rows<T, NV, 4>(st, v, a);
+      fold_rows<T, NV, true>(st, v, a);
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if (t + k * a.tpr < vecs) {
           const Vec16 one[1] = {v[k]};
-          fold_rows<T, 1, 4>(st, one, a);
+          fold_rows<T, 1, true>(st, one, a);
         }
       }
     }
@@ -708,17 +748,21 @@ __global__ void __launch_bounds__(512) policy_short_kernel(const __grid_constant
   const float gm = group_reduce<MaxOp>(st.m, red[0], nw, first_warp);
   const float gs = group_reduce<SumOp>(merged(st, gm, a), red[1], nw, first_warp);
   if (r >= a.M) return;
-  if (t == 0) write_row<kPolicy>(a, pol, o, r, col >= 0, xl, gm, gs);
+  const RowStat rs(gm, gs, a);
+  if (t == 0) write_row<kPolicy>(a, pol, o, r, col >= 0, xl, rs);
   if (col < 0) {
     zero_row<T>(yr, a.N, t, a.tpr);
     return;
   }
-  const RowStat rs(gm, gs, a);
   const double logp = rs.logp(a, xl);
   const GradTerms gt = grad_terms(rs, a, dl, policy_row(pol, r, logp).g);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if (t + k * a.tpr < vecs) grad_vec<T>(v[k], gt, yr + static_cast<int64_t>(t + k * a.tpr) * E);
+    if (t + k * a.tpr < vecs) {
+      T* y = yr + static_cast<int64_t>(t + k * a.tpr) * E;
+      if (gt.far) grad_vec<T, true>(v[k], gt, y);
+      else grad_vec<T, false>(v[k], gt, y);
+    }
   if (static_cast<int>(col / E % a.tpr) == t) yr[col] = from_f<T>(gt.k1 * expm1f(static_cast<float>(logp)));
 }
 

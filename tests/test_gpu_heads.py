@@ -61,7 +61,7 @@ def check_backward(out, dq, dk, q, k, qw, kw, phi, inter):
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("d,rot", [(128, 128), (64, 64), (256, 256), (80, 40), (72, 72), (96, 96), (128, 32), (576, 64),
-                                   (40, 8), (36, 20), (5, 4), (2, 2), (33, 32), (1024, 1024)])
+                                   (40, 8), (36, 20), (5, 4), (2, 2), (33, 32), (1024, 1024), (72, 36), (200, 100), (8, 4), (16, 12)])
 def test_head_sizes(d, rot, inter, dt):
     check_all((7, 9), 5, 2, d, rot, dt, inter)
 
