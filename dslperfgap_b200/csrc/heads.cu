@@ -32,8 +32,10 @@
 // formed its own angles; the addresses, bounds and waits of that took 200 of 440
 // instructions a group of rows: forward 61.0 us against
 // 59.5 for 16384 tokens of 32 + 8 heads of 128 in bf16 (the same bytes copied by
-// cudaMemcpy's kernel: 58), the rotation of 29971 tokens of 16 + 16 heads 86.8
-// against 86.0 (81.5), and one decoded token 6.2 against 4.2.
+// cudaMemcpy's kernel: 58), backward 108 against 90, the rotation of 29971 tokens
+// of 16 + 16 heads 86.8 against 82 (81.5), and one decoded token 6.2 against 4.2.
+#include <algorithm>
+
 #include "common.cuh"
 #include "pipe.cuh"
 
@@ -65,6 +67,7 @@ struct HeadArgs {
   int stages, stage_bytes, row_bytes;
   int angle_warps, row_warps;
   int groups;          // groups of a tile: those of q's rows, then those of k's (the last ones may be empty)
+  int q_groups, q_warps;  // norm backward: groups of q's rows in every tile, and the row warps that take them
   // From a tile of a CTA to its next one (parts == 1): tokens modulo seq; what is
   // added to a token's place in x, dy and pos, and once more where a sequence ends.
   uint32_t s_step;
@@ -245,18 +248,18 @@ DSLPG_DEV void turn(float (&fa)[V], float (&fb)[V], const float4* angles, int ro
 
 // Parts of a CTA's dynamic shared memory, in this order.
 struct HeadSmem {
-  int stages, stage_bytes, angle_bytes, n, weight_floats, other_bytes;
+  int stages, stage_bytes, angle_bytes, n, weight_floats, sum_bytes;
   __host__ __device__ int angles() const { return stages * stage_bytes; }            // [stages][tt][planes]
   __host__ __device__ int freq() const { return angles() + stages * angle_bytes; }   // uint64 [n]
   __host__ __device__ int weight() const { return (freq() + 8 * n + 15) & ~15; }     // [2][weight_floats]
-  __host__ __device__ int other() const { return weight() + 8 * weight_floats; }     // [row threads][2 V] floats
-  __host__ __device__ int bars() const { return other() + other_bytes; }
+  __host__ __device__ int sums() const { return weight() + 8 * weight_floats; }      // [row warps][D] floats
+  __host__ __device__ int bars() const { return sums() + sum_bytes; }
   __host__ __device__ int total() const { return bars() + 16 * stages; }
 };
 
-__host__ __device__ inline HeadSmem head_smem(const HeadArgs& a, int op, int V) {
+__host__ __device__ inline HeadSmem head_smem(const HeadArgs& a, int op) {
   return HeadSmem{a.stages, a.stage_bytes, (a.tt * a.n * 8 + 15) & ~15, a.n, op == kRotate ? 0 : (a.D + 3) & ~3,
-                  op == kNormBwd ? a.row_warps * 32 * 2 * V * 4 : 0};
+                  op == kNormBwd ? (a.row_warps * a.D * 4 + 15) & ~15 : 0};
 }
 
 // A tile: tokens [token, token + count), heads [lo, lo + n) of either tensor.
@@ -305,17 +308,25 @@ struct Place {
     }
   }
 };
-// Threads of a CTA, by HeadOp: 6 warps (80 registers each) and 5 (96) on each of an SM's four schedulers.
-constexpr int kTileThreads[3] = {768, 768, 640};
+// Threads of a CTA at most. Whole 16-byte vectors need few warps, and more of them
+// disturb one another's streams; narrower ones need the instruction slots. Measured
+// (us) with 512, 640 and 768 threads: rotation of 29971 tokens of 16 + 16 heads of
+// 128 in bf16 81.9, 83.9, 86.0, of 6845 of 16 + 16 of 72 in fp16 22.6, 20.6, 19.1;
+// norm of 16384 tokens of 32 + 8 of 128 in bf16 65.7, 59.6, 59.5; its backward 90.0,
+// 99.0, 119.
+constexpr int tile_threads(int op, bool whole) {
+  return op == kNorm ? 768 : (op == kRotate ? (whole ? 512 : 768) : (whole ? 512 : 640));
+}
+template <typename T, int V> constexpr bool kWholeVec = V == Elt<T>::kPerVec;
 
 template <typename T, int V, bool INTER, int OP>
-__global__ void __launch_bounds__(kTileThreads[OP], 1)
+__global__ void __launch_bounds__(tile_threads(OP, kWholeVec<T, V>), 1)
     heads_tile_kernel(const __grid_constant__ HeadArgs a, unsigned long long limit_ns) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ volatile int abort_flag;
   constexpr int kBytes = Pack<T, V>::kBytes;
   constexpr bool NORM = OP != kRotate, BWD = OP == kNormBwd;
-  const HeadSmem lay = head_smem(a, OP, V);
+  const HeadSmem lay = head_smem(a, OP);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int vecs = a.D / V;
   uint64_t* freq = reinterpret_cast<uint64_t*>(smem + lay.freq());
@@ -456,32 +467,20 @@ __global__ void __launch_bounds__(kTileThreads[OP], 1)
   const Lane<INTER> ln(a, lane);
   const bool rotated = ln.active && ln.u < a.rot_units;
   const int b_off = (ln.ib - ln.ia) * V, b_bytes = b_off * static_cast<int>(sizeof(T));
-  float da[V], db[V];  // norm backward: dw sums of the tensor in hand; the other's in shared memory
-  float4* other = reinterpret_cast<float4*>(smem + lay.other()) + me * 32 + lane;
-  const int others = a.row_warps * 32;
-  auto exchange = [&] {
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
-      const float4 f = other[e * others];
-      other[e * others] = make_float4(da[2 * e], da[2 * e + 1], db[2 * e], db[2 * e + 1]);
-      da[2 * e] = f.x;
-      da[2 * e + 1] = f.y;
-      db[2 * e] = f.z;
-      db[2 * e + 1] = f.w;
-    }
-  };
-  bool in_hand = false;
+  float da[V], db[V];  // norm backward: this lane's dw sums; a warp takes the rows of one tensor
   if constexpr (BWD) {
 #pragma unroll
     for (int e = 0; e < V; ++e) da[e] = db[e] = 0.f;
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) other[e * others] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  const bool of_k = BWD && me >= a.q_warps;
 
-  // Group g of the CTA's it-th tile: the groups of all its tiles go round the row warps, and a warp waits for those
-  // tiles alone that hold one of its groups. A stage is free when all its groups are done.
+  // Group g of the CTA's it-th tile: the groups of all its tiles go round the row warps (norm backward: q's and k's round
+  // their own), and a warp waits for those tiles alone that hold one of its groups. A stage is free when all its groups
+  // are done.
   uint32_t st = 0, phase = 0, tile = blockIdx.x;
-  int g = me;  // row_warps <= groups
+  const int g_end = BWD && !of_k ? a.q_groups : a.groups, g_begin = of_k ? a.q_groups : 0;
+  const int g_step = BWD ? (of_k ? a.row_warps - a.q_warps : a.q_warps) : a.row_warps;
+  int g = of_k ? me - a.q_warps + a.q_groups : me;  // < g_end: no more warps than groups
   bool fresh = true;
   uint32_t base = 0;
   const float4* table = nullptr;
@@ -495,21 +494,16 @@ __global__ void __launch_bounds__(kTileThreads[OP], 1)
       table = reinterpret_cast<const float4*>(smem + lay.angles() + st * lay.angle_bytes);
       rows_q = t.rows[0];
       rows_k = t.rows[1];
-      q_groups = (rows_q + a.rpw - 1) / a.rpw;
+      q_groups = BWD ? a.q_groups : (rows_q + a.rpw - 1) / a.rpw;
       out_q = static_cast<T*>(a.y[0]) + (static_cast<int64_t>(t.token) * a.heads[0] + t.lo[0]) * a.D + ln.ia * V;
       out_k = static_cast<T*>(a.y[1]) + (static_cast<int64_t>(t.token) * a.heads[1] + t.lo[1]) * a.D + ln.ia * V;
     }
     {
-      const bool seg = g >= q_groups;
+      const bool seg = BWD ? of_k : g >= q_groups;
       int r = (seg ? g - q_groups : g) * a.rpw + ln.sub;
       const bool ok = ln.active && r < (seg ? rows_k : rows_q);
       int row = r + (seg ? rows_q : 0);  // in the stage
       if (!ok) r = row = 0;
-      if constexpr (BWD)
-        if (seg != in_hand) {
-          exchange();
-          in_hand = seg;
-        }
       const uint32_t src = base + row * a.row_bytes + ln.ia * kBytes;
       const uint32_t magic = seg ? a.magic[1] : a.magic[0];
       const int k = magic ? __umulhi(r, magic) : r;  // the row's token
@@ -581,10 +575,10 @@ __global__ void __launch_bounds__(kTileThreads[OP], 1)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + 8 * st);
-    g += a.row_warps;
-    fresh = g >= a.groups;
-    while (g >= a.groups) {
-      g -= a.groups;
+    g += g_step;
+    fresh = g >= g_end;
+    while (g >= g_end) {
+      g -= g_end - g_begin;
       tile += gridDim.x;
       if (++st == static_cast<uint32_t>(a.stages)) {
         st = 0;
@@ -594,43 +588,27 @@ __global__ void __launch_bounds__(kTileThreads[OP], 1)
   }
 
   if constexpr (BWD) {
-    // dw: the rows of a group, then the warps (through the stages, which are done with), then (heads_dw_kernel) the CTAs,
-    // each in a fixed order, so that the same call gives the same bits
-    auto rows_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(others) : "memory"); };
-    if (in_hand) exchange();
-    float* sums = reinterpret_cast<float*>(smem + lay.other());
-    float keep[2][2][V];
+    // dw: the rows of a group, then the tensor's warps, then (heads_dw_kernel) the CTAs, each in a fixed order, so that
+    // the same call gives the same bits
+    float* sums = reinterpret_cast<float*>(smem + lay.sums());  // [row warps][D]
 #pragma unroll
-    for (int seg = 0; seg < 2; ++seg) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float ta = da[e], tb = db[e];
-        for (int r = 1; r < a.rpw; ++r) {
-          ta += __shfl_sync(0xffffffffu, da[e], (ln.u + r * a.units) & 31);
-          tb += __shfl_sync(0xffffffffu, db[e], (ln.u + r * a.units) & 31);
-        }
-        keep[seg][0][e] = ta;
-        keep[seg][1][e] = tb;
+    for (int e = 0; e < V; ++e) {
+      float ta = da[e], tb = db[e];
+      for (int r = 1; r < a.rpw; ++r) {
+        ta += __shfl_sync(0xffffffffu, da[e], (ln.u + r * a.units) & 31);
+        tb += __shfl_sync(0xffffffffu, db[e], (ln.u + r * a.units) & 31);
       }
-      exchange();
-    }
-    rows_sync();  // every lane's own slots are read; they become [row warps][D] sums
-#pragma unroll
-    for (int seg = 0; seg < 2; ++seg) {
       if (ln.active && ln.sub == 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          sums[me * a.D + ln.ia * V + e] = keep[seg][0][e];
-          sums[me * a.D + ln.ib * V + e] = keep[seg][1][e];
-        }
+        sums[me * a.D + ln.ia * V + e] = ta;
+        sums[me * a.D + ln.ib * V + e] = tb;
       }
-      rows_sync();
-      for (int d = me * 32 + lane; d < a.D; d += others) {
-        float t = 0.f;
-        for (int k = 0; k < a.row_warps; ++k) t += sums[k * a.D + d];
-        a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + seg) * a.D + d] = t;
-      }
-      rows_sync();
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(a.row_warps * 32) : "memory");
+    for (int i = me * 32 + lane; i < 2 * a.D; i += a.row_warps * 32) {
+      const int seg = i >= a.D, d = i - seg * a.D;
+      float t = 0.f;
+      for (int k = seg ? a.q_warps : 0; k < (seg ? a.row_warps : a.q_warps); ++k) t += sums[k * a.D + d];
+      a.partial[static_cast<int64_t>(blockIdx.x) * 2 * a.D + i] = t;
     }
   }
 }
@@ -781,8 +759,8 @@ uint32_t magic_of(int heads) { return heads > 1 ? static_cast<uint32_t>(((1ull <
 // 40 KB), fewer tokens while that leaves SMs without four tiles each, and less
 // than a token where one token is too large or there are not tokens enough.
 // Measured (us) with 20, 40 and 80 KB: norm forward of 16384 tokens of 32 + 8
-// heads of 128 in bf16 90.2, 61.6, 59.5 (its backward 147, 113, 107); rotation of
-// 29971 tokens of 16 + 16 heads 135, 86.0, 90.8.
+// heads of 128 in bf16 90.2, 61.6, 59.5; rotation of 29971 tokens of 16 + 16 heads
+// 135, 86.0, 90.8 (with 768 threads).
 template <typename T> void set_tiles(HeadArgs& a, int op) {
   const int heads = a.heads[0] + a.heads[1], copies = op == kNormBwd ? 2 : 1, sms = sm_count();
   a.row_bytes = a.D * static_cast<int>(sizeof(T));
@@ -816,18 +794,29 @@ cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   a.units = a.D / (2 * V);
   a.rpw = 32 / a.units;
   set_tiles<T>(a, OP);
-  a.groups = a.parts == 1 ? (a.heads[0] * a.tt + a.rpw - 1) / a.rpw + (a.heads[1] * a.tt + a.rpw - 1) / a.rpw
-                          : (a.part + a.rpw - 1) / a.rpw + 1;
+  const int part_groups = (a.part + a.rpw - 1) / a.rpw;
+  a.q_groups = a.parts == 1 ? (a.heads[0] * a.tt + a.rpw - 1) / a.rpw : part_groups;
+  const int k_groups = a.parts == 1 ? (a.heads[1] * a.tt + a.rpw - 1) / a.rpw : (OP == kNormBwd ? part_groups : 1);
+  a.groups = a.q_groups + k_groups;
   // Warps: one for copies; some for angles; the rest for rows, no more than a tile has groups. One angle warp for two
-  // tokens (backward, whose rows take twice the time: for four; 107.4 us against 110.7 for the training batch above).
+  // tokens (backward, whose rows take twice the time: for four).
   a.angle_warps = OP == kNormBwd ? (a.tt + 3) / 4 : (a.tt + 1) / 2;
-  a.row_warps = kTileThreads[OP] / 32 - 1 - a.angle_warps;
+  a.row_warps = tile_threads(OP, kWholeVec<T, V>) / 32 - 1 - a.angle_warps;
   if (a.row_warps > a.groups) a.row_warps = a.groups;
+  // The q : k split of the row warps that ends first: the largest share of groups a warp, as fractions over the other's
+  // warps. Exchanging the sums of two tensors in one warp took 50 instructions a time instead.
+  a.q_warps = k_groups ? (a.q_groups ? 1 : 0) : a.row_warps;
+  auto longer = [&](int q) {
+    const int k = a.row_warps - q;
+    return std::max(q ? a.q_groups * 1.0 / q : (a.q_groups ? 1e9 : 0.0), k ? k_groups * 1.0 / k : (k_groups ? 1e9 : 0.0));
+  };
+  for (int q = a.q_warps + 1; q <= a.row_warps; ++q)
+    if (longer(q) < longer(a.q_warps)) a.q_warps = q;
   const int block = 32 * (1 + a.angle_warps + a.row_warps);
   const void* fn = reinterpret_cast<const void*>(&heads_tile_kernel<T, V, INTER, OP>);
   const int grid = static_cast<int>(a.tiles < static_cast<uint32_t>(sm_count()) ? a.tiles : sm_count());
   const int mine = static_cast<int>((a.tiles + grid - 1) / grid);  // tiles of a CTA at most
-  for (a.stages = mine < 16 ? mine : 16; a.stages > 1 && head_smem(a, OP, V).total() > kTileSmem; --a.stages) {
+  for (a.stages = mine < 16 ? mine : 16; a.stages > 1 && head_smem(a, OP).total() > kTileSmem; --a.stages) {
   }
   const int64_t ahead = static_cast<int64_t>(grid) * a.tt, db = ahead / a.seq, ds = ahead % a.seq;
   for (int seg = 0; seg < 2; ++seg) {
@@ -839,7 +828,7 @@ cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   a.p_step = db * a.ps[1] + ds * a.ps[2];
   a.p_carry = a.ps[1] - static_cast<int64_t>(a.seq) * a.ps[2];
   a.s_step = static_cast<uint32_t>(ds);
-  const size_t smem = head_smem(a, OP, V).total();
+  const size_t smem = head_smem(a, OP).total();
   if (cudaError_t e = allow_dynamic_smem(fn, smem)) return e;
   heads_tile_kernel<T, V, INTER, OP><<<grid, block, smem, st>>>(a, kWaitLimitNs);
   if (cudaError_t e = cudaGetLastError()) return e;
