@@ -432,6 +432,25 @@ unsigned int take_wait_timeouts_rowstat();
 unsigned int take_wait_timeouts_ff();
 unsigned int take_wait_timeouts_heads();
 
+// A small kernel that works on the results of the launch before it in its stream:
+// its launch overlaps that one's end (programmatic dependent launch), and
+// wait_for_primary(), its first statement, holds it until those results are there.
+DSLPG_DEV void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int block, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 inline int dtype_size(int dt) { return dt == DSLPG_F32 ? 4 : 2; }
 inline bool is_float_dtype(int dt) { return dt == DSLPG_F32 || dt == DSLPG_F16 || dt == DSLPG_BF16; }
 inline bool aligned(const void* p, int bytes) {

@@ -637,6 +637,7 @@ struct Cursor {
 // dw[seg][d] = the sum of the CTAs' partial rows: 8 threads a column, each every 8th row, merged in order.
 __global__ void __launch_bounds__(256) heads_dw_kernel(const float* partial, int ctas, int D, float* dq, float* dk) {
   __shared__ float part[8][32];
+  wait_for_primary();
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + col, seg = blockIdx.y;
   float t = 0.f;
@@ -832,8 +833,8 @@ cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   if (cudaError_t e = allow_dynamic_smem(fn, smem)) return e;
   heads_tile_kernel<T, V, INTER, OP><<<grid, block, smem, st>>>(a, kWaitLimitNs);
   if (cudaError_t e = cudaGetLastError()) return e;
-  if constexpr (OP == kNormBwd) heads_dw_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, grid, a.D, dwq, dwk);
-  return cudaGetLastError();
+  if constexpr (OP == kNormBwd) return launch_dependent(heads_dw_kernel, dim3((a.D + 31) / 32, 2), 256, st, static_cast<const float*>(a.partial), grid, a.D, dwq, dwk);
+  return cudaSuccess;
 }
 
 template <typename T, bool NORM, bool BWD>
@@ -847,8 +848,8 @@ cudaError_t launch_any(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   if (BWD && grid > kPartialRows) grid = kPartialRows;
   heads_any_kernel<T, NORM, BWD><<<grid, kAnyBlock, smem, st>>>(a);
   if (cudaError_t e = cudaGetLastError()) return e;
-  if constexpr (BWD) heads_dw_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, grid, a.D, dwq, dwk);
-  return cudaGetLastError();
+  if constexpr (BWD) return launch_dependent(heads_dw_kernel, dim3((a.D + 31) / 32, 2), 256, st, static_cast<const float*>(a.partial), grid, a.D, dwq, dwk);
+  return cudaSuccess;
 }
 
 // Whether rows can be cut into units of two V-element vectors.

@@ -382,6 +382,7 @@ DSLPG_DEV double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x)))
 __global__ void __launch_bounds__(256) pair_kernel(const LossRows a, const PairTerms p, const float* logp, float* loss,
                                                    float* log_ratio) {
   __shared__ double part[2][8];
+  wait_for_primary();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t k = blockIdx.x; k < p.pairs; k += gridDim.x) {
     for (int side = 0; side < 2; ++side) {
@@ -997,8 +998,8 @@ extern "C" int dslpg_preference_loss_fwd(const dslpg_logit_rows* rows, const dsl
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   const int grid = static_cast<int>(p.pairs < 65535 ? p.pairs : 65535);
-  pair_kernel<<<grid, 256, 0, stream>>>(a, p, logp, loss, log_ratio);
-  return static_cast<int>(cudaGetLastError());
+  return static_cast<int>(
+      launch_dependent(pair_kernel, dim3(grid), 256, stream, a, p, static_cast<const float*>(logp), loss, log_ratio));
 }
 
 extern "C" int dslpg_preference_loss_bwd(const dslpg_logit_rows* rows, const dslpg_pair_terms* terms,
