@@ -30,10 +30,10 @@
 // tensor, so a row's place in both is its number, and a group may span tokens.
 // Before this, each warp copied its own rows (cp.async, one lane a vector) and
 // formed its own angles; the addresses, bounds and waits of that took 200 of 440
-// instructions a group of rows: forward 61.0 us against
-// 59.5 for 16384 tokens of 32 + 8 heads of 128 in bf16 (the same bytes copied by
-// cudaMemcpy's kernel: 58), backward 108 against 90, the rotation of 29971 tokens
-// of 16 + 16 heads 86.8 against 82 (81.5), and one decoded token 6.2 against 4.2.
+// instructions a group of rows: forward 61.0 us against 59.5 for 16384 tokens of
+// 32 + 8 heads of 128 in bf16 (a torch copy of the same bytes: 58), backward 108
+// against 90, the rotation of 29971 tokens of 16 + 16 heads 86.8 against 82
+// (81.5), and one decoded token 6.2 against 4.2.
 #include <algorithm>
 
 #include "common.cuh"
@@ -66,6 +66,7 @@ struct HeadArgs {
   uint32_t tiles;
   int stages, stage_bytes, row_bytes;
   int angle_warps, row_warps;
+  int pairs;           // an angle warp forms two tokens' angles side by side
   int groups;          // groups of a tile: those of q's rows, then those of k's (the last ones may be empty)
   int q_groups, q_warps;  // norm backward: groups of q's rows in every tile, and the row warps that take them
   // From a tile of a CTA to its next one (parts == 1): tokens modulo seq; what is
@@ -368,6 +369,12 @@ __global__ void __launch_bounds__(tile_threads(OP, kWholeVec<T, V>), 1)
     const int64_t step = is_dy ? a.dy_step[seg] : a.x_step[seg], carry = is_dy ? a.dy_carry[seg] : a.x_carry[seg];
     const bool joined = st_h == a.D || a.heads[seg] == 1;  // heads that follow one another go in one copy
     const bool all_joined = __all_sync(0xffffffffu, joined || !mine);
+    // Small tokens that follow one another too: one copy of them all, as the copy engine takes some 90 cycles for each
+    // (99147 tokens of 4 + 1 heads of 64: 61.6 us against 75.9 with a copy a token). Larger ones are better apart (6845
+    // tokens of 16 + 16 of 72 in fp16: 18.5 against 20.1).
+    const int token_bytes = a.heads[seg] * a.row_bytes;
+    const bool dense = all_joined && token_bytes <= 1024 && st_s == static_cast<int64_t>(a.heads[seg]) * a.D &&
+                       (a.tokens <= a.seq || st_b == a.seq * st_s);
     Place place;
     uint32_t it = 0, st = 0, phase = 0;
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++it) {
@@ -379,7 +386,7 @@ __global__ void __launch_bounds__(tile_threads(OP, kWholeVec<T, V>), 1)
       const uint32_t bar = full + 8 * st;
       const uint32_t dst = stage0 + st * a.stage_bytes +
                            ((is_dy ? t.rows[0] + t.rows[1] : 0) + (seg ? t.rows[0] : 0) + k * heads) * a.row_bytes;
-      const bool ok = mine && k < t.count && heads > 0;
+      const bool ok = mine && k < (dense ? 1 : t.count) && heads > 0;
       if (it >= static_cast<uint32_t>(a.stages) && !wait(empty + 8 * st, phase ^ 1u)) break;
       if (lane == 0) mbar_arrive_expect_tx(bar, (t.rows[0] + t.rows[1]) * a.row_bytes * (BWD ? 2 : 1));
       __syncwarp();
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(tile_threads(OP, kWholeVec<T, V>), 1)
                      : "memory");
       };
       if (all_joined) {
-        if (ok) copy(dst, src, heads * a.row_bytes);
+        if (ok) copy(dst, src, (dense ? t.count : 1) * heads * a.row_bytes);
       } else {
         for (int j = 0; j < (BWD ? 32 : 16); ++j) {  // a row a lane, token by token
           const int n = __shfl_sync(0xffffffffu, ok ? heads : 0, j);
@@ -440,14 +447,30 @@ __global__ void __launch_bounds__(tile_threads(OP, kWholeVec<T, V>), 1)
         }
         const int count = Tile(a, tile).count;
         float2* table = reinterpret_cast<float2*>(smem + lay.angles() + st * lay.angle_bytes);
-        for (int k = warp - 1, j = 0; k < count; k += a.angle_warps, ++j)
-#pragma unroll 2
-          for (int i0 = 0; i0 < a.n; i0 += 32) {
-            const int i = i0 + lane;
-            const int64_t at = __shfl_sync(0xffffffffu, ahead[q], 4 * j + axis_of(a, i));
-            if (i < a.n)
-              table[k * a.n + angle_slot<V>(i, a.rot_units)] = angle_of<sizeof(T) == 4>(at, freq[i], a.sign);
+        if (a.pairs) {
+          for (int k = warp - 1, j = 0; k < count; k += 2 * a.angle_warps, j += 2) {
+            const bool two = k + a.angle_warps < count;
+#pragma unroll 1
+            for (int i0 = 0; i0 < a.n; i0 += 32) {
+              const int i = min(i0 + lane, a.n - 1), from = 4 * j + axis_of(a, i);
+              const int64_t p0 = __shfl_sync(0xffffffffu, ahead[q], from), p1 = __shfl_sync(0xffffffffu, ahead[q], from + 4);
+              const uint64_t f = freq[i];
+              const float2 c0 = angle_of<sizeof(T) == 4>(p0, f, a.sign), c1 = angle_of<sizeof(T) == 4>(p1, f, a.sign);
+              float2* to = table + k * a.n + angle_slot<V>(i, a.rot_units);
+              *to = c0;  // (lanes past the last frequency write its value too)
+              if (two) to[a.angle_warps * a.n] = c1;
+            }
           }
+        } else {
+          for (int k = warp - 1, j = 0; k < count; k += a.angle_warps, ++j)
+#pragma unroll 2
+            for (int i0 = 0; i0 < a.n; i0 += 32) {
+              const int i = i0 + lane;
+              const int64_t at = __shfl_sync(0xffffffffu, ahead[q], 4 * j + axis_of(a, i));
+              if (i < a.n)
+                table[k * a.n + angle_slot<V>(i, a.rot_units)] = angle_of<sizeof(T) == 4>(at, freq[i], a.sign);
+            }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8 * st);
         ahead[q] = position(tile + kAhead * gridDim.x, false);
@@ -795,6 +818,7 @@ cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   a.units = a.D / (2 * V);
   a.rpw = 32 / a.units;
   set_tiles<T>(a, OP);
+  const int heads = a.heads[0] + a.heads[1];
   const int part_groups = (a.part + a.rpw - 1) / a.rpw;
   a.q_groups = a.parts == 1 ? (a.heads[0] * a.tt + a.rpw - 1) / a.rpw : part_groups;
   const int k_groups = a.parts == 1 ? (a.heads[1] * a.tt + a.rpw - 1) / a.rpw : (OP == kNormBwd ? part_groups : 1);
@@ -802,8 +826,17 @@ cudaError_t launch_tile(HeadArgs a, float* dwq, float* dwk, cudaStream_t st) {
   // Warps: one for copies; some for angles; the rest for rows, no more than a tile has groups. One angle warp for two
   // tokens (backward, whose rows take twice the time: for four).
   a.angle_warps = OP == kNormBwd ? (a.tt + 3) / 4 : (a.tt + 1) / 2;
+  // An angle is a chain of a few hundred cycles, so two tokens' run side by side, but not in a rotation whose rows weigh
+  // more (16 whole heads of 16-bit elements a token): there the slower angles keep the loads and stores of all SMs in a
+  // better order; why was not found. Single / pairs, in us, for 45000 tokens in bf16 of 6 + 6 heads of 128: 57.7 / 51.3,
+  // of 8 + 4 of 256: 140 / 103, of 8 + 8 of 128: 63.7 / 71.2, of 16 + 16: 121 / 143; 99147 in float32 of 8 + 8 of 128:
+  // 265 / 295.
+  a.pairs = OP != kRotate || static_cast<int64_t>(heads) * a.row_bytes < 64ll * a.n;
   a.row_warps = tile_threads(OP, kWholeVec<T, V>) / 32 - 1 - a.angle_warps;
-  if (a.row_warps > a.groups) a.row_warps = a.groups;
+  if (a.row_warps > a.groups) {  // (4 + 1 heads of 96, 99147 tokens: norm 113 us without the spare warps, 90 with them)
+    a.angle_warps = std::min(a.tt, a.angle_warps + a.row_warps - a.groups);
+    a.row_warps = a.groups;
+  }
   // The q : k split of the row warps that ends first: the largest share of groups a warp, as fractions over the other's
   // warps. Exchanging the sums of two tensors in one warp took 50 instructions a time instead.
   a.q_warps = k_groups ? (a.q_groups ? 1 : 0) : a.row_warps;
