@@ -282,3 +282,23 @@ def test_guard_bytes_around_outputs():
             assert (b[:256] == 0xA5).all() and (b[-256:] == 0xA5).all()
         want = B.qk_norm_rope_bwd(q, k, q, k, qw, kw, pos, freq, eps=EPS)
         assert torch.equal(bufs[0][256:-256], want[0].view(-1).view(torch.uint8))
+
+
+@pytest.mark.parametrize("axes", [1, 4])
+@pytest.mark.parametrize("hq,hk,d,dt", [(1, 1, 64, "bf16"), (4, 1, 96, "f16"), (1, 4, 72, "f32")])
+def test_few_heads_many_tokens(hq, hk, d, dt, axes):
+    """Tiles of 8 tokens, several of a tile in one copy where they follow one another, and not where a sequence ends
+    (an odd length) or the batches lie apart: the same bits each way."""
+    check_all((2, 5003), hq, hk, d, d, dt, axes=axes)
+    q, k, qw, kw, pos, freq, sec = make((2, 5003), hq, hk, d, d, dt, axes=axes)
+    apart = [torch.zeros(2, 5010, *x.shape[2:], dtype=x.dtype, device="cuda") for x in (q, k)]
+    for a, x in zip(apart, (q, k)):
+        a[:, :5003] = x
+    q2, k2 = (a[:, :5003] for a in apart)
+    ways = [(q, k), (q2, k2), (q, k2)]
+    for f in (lambda a, b: B.qk_norm_rope(a, b, qw, kw, pos, freq, sections=sec),
+              lambda a, b: B.rope(a, b, pos, freq, sections=sec),
+              lambda a, b: B.qk_norm_rope_bwd(q, k, a, b, qw, kw, pos, freq, sections=sec)):
+        first = f(*ways[0])
+        for way in ways[1:]:
+            assert all(torch.equal(g, w) for g, w in zip(f(*way), first))
