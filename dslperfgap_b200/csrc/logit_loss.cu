@@ -251,7 +251,7 @@ template <typename T> struct Stretch {
 };
 
 // Fold elements [0, n) from xr on with `tpr` threads, this one being t: 16-byte
-// vectors, the next ones loaded before this round's arithmetic, and the elements
+// vectors, the next ones loaded before this step's arithmetic, and the elements
 // before the first and behind the last whole vector, one a thread.
 template <typename T, int U, bool PACKED, class Load>
 DSLPG_DEV void fold_row(Stat& st, const T* xr, int64_t n, const LossRows& a, int t, int tpr, Load ld) {
