@@ -12,10 +12,14 @@
 //
 // Angles: as fractions of a turn in 64-bit fixed point, where f_i / 2 pi times an
 // integer position is one wrapping integer product: the whole turns fall off
-// exactly, for negative and far positions (1e6 and more) alike, and the cosine
-// keeps its 32-bit accuracy. (The same in double precision took 0.9 us a token
-// in its warp, a chain of conversions and roundings.) The n angles of a token
-// are formed once and serve all of its heads.
+// exactly, for negative and far positions alike. f_i / 2 pi is right to its last
+// bit for |f_i| up to 2^18, so an angle is off by |position| 2^-64 turns beside its
+// own rounding, and the cosine keeps its 32-bit accuracy for positions up to 2^38.
+// (A further 32 bits, for tiles that hold a position beyond 32 bits alone, would
+// reach every int64 position, but the test for such tiles took 3 to 7 % of tokens
+// of few heads; the whole in double precision took 0.9 us a token in its warp, a
+// chain of conversions and roundings.) The n angles of a token are formed once and
+// serve all of its heads.
 //
 // Lanes: a row is cut into units of two V-element vectors that hold both
 // members of V rotated pairs (vectors u and u + n/V; interleaved 2u and
@@ -106,15 +110,22 @@ template <typename T, int V> DSLPG_DEV void st_vec(T* dst, const float (&f)[V]) 
   else StoreOut<T, V>::run(dst, f);
 }
 
-// The part of a turn that one position step makes, in units of 2^-64 turns.
+// The part of a turn that one position step makes, in units of 2^-64 turns, rounded to the nearest. 1 / (2 pi) is taken
+// in two parts, as one double's rounding (2^-55 |f| turns) shows at positions of 2^31: the first has 29 bits, so that
+// its product with a float32 is exact, the second's is off by less than 2^-83 |f|.
 DSLPG_DEV uint64_t turn_per_step(float f) {
-  const double turns = static_cast<double>(f) * 0.15915494309189533577;  // 1 / (2 pi)
-  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+  const double size = fabs(static_cast<double>(f));
+  auto fraction = [](double turns) { return (turns - floor(turns)) * 0x1p64; };
+  const double a = fraction(size * 0x1.45f306dp-3), b = fraction(size * 0x1.9391054a7f09dp-32);
+  const uint64_t whole_a = static_cast<uint64_t>(a), whole_b = static_cast<uint64_t>(b);
+  const double rest = (a - static_cast<double>(whole_a)) + (b - static_cast<double>(whole_b));
+  const uint64_t step = whole_a + whole_b + static_cast<uint64_t>(rest + 0.5);
+  return f < 0.f ? 0 - step : step;
 }
 
 // Cosine and sine (times `sign`) of position p at a frequency's turn_per_step.
-// For 16-bit rows the SFU's, off by at most 2^-20.9 on this range, far inside
-// the rows' own rounding (2^-12, 2^-9) and a fifth of the instructions.
+// For 16-bit rows the SFU's, a fifth of the instructions: off by at most 2^-19.9 (2^-21.2 its own on -pi .. pi, and the
+// argument's three roundings of pi 2^-24), far inside the rows' own rounding (2^-12, 2^-9).
 template <bool EXACT> DSLPG_DEV float2 angle_of(int64_t p, uint64_t step, float sign) {
   const int turn = static_cast<int>((static_cast<uint64_t>(p) * step) >> 32);  // 2^-32 turns, -2^31 .. 2^31
   float sn, cn;

@@ -9,8 +9,8 @@ q and k are ``[tokens, heads, head_dim]`` or ``[batch, seq, heads, head_dim]``
 (any strides with a dense last axis, so views into one projection output are
 read in place); outputs are dense. ``inv_freq`` (float32, n values) rotates the
 first 2n features: pairs (i, i + n), or (2i, 2i + 1) when ``interleaved``; the
-others pass through; it has to be finite. ``positions`` (int32 or int64) has q's token axes, or
-broadcasts to them. With ``sections`` (one to four counts that add up to n) it
+others pass through; it has to be finite. Angles are right to fp32 for positions up to 2^38 in size
+(and |inv_freq| up to 2^18). ``positions`` (int32 or int64) has q's token axes, or broadcasts to them. With ``sections`` (one to four counts that add up to n) it
 has one more leading axis, and frequency i turns by the axis whose section
 holds i: time, height and width of video patches, for instance.
 """

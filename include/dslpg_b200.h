@@ -316,8 +316,10 @@ DSLPG_API int dslpg_kernel_ff_static(const void* x, const void* w1, const void* 
  *   u = x / sqrt(mean(x^2) + eps) * weight            (rope: u = x)
  *   y_i = u_i cos phi_i - u_j sin phi_i;   y_j = u_j cos phi_i + u_i sin phi_i
  * and the features past rotary_dim are u. Arithmetic is fp32 with one rounding
- * at the store; the angles are formed in 64 bits, so that far positions keep
- * the cosine to fp32 accuracy.
+ * at the store. The angles are formed in 64-bit fixed point, off by
+ * |position| 2^-64 turns for |inv_freq| up to 2^18 (which have to be finite):
+ * positions up to 2^38 in size keep the cosine to fp32 accuracy, those up to
+ * 2^50 to 4e-4.
  *
  * `positions` (int32 or int64) has `axes` (1 to 4) values for each token, with
  * axis, batch and seq strides (0: broadcast). Frequency i turns by axis a where
