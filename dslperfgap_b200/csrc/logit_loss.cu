@@ -200,7 +200,8 @@ struct PolicyRow {
 };
 
 DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, float old_logp, float adv, float ref, double logp) {
-  const float ratio = expf(static_cast<float>(logp - static_cast<double>(old_logp)));
+  float ratio = expf(static_cast<float>(logp - static_cast<double>(old_logp)));
+  if (adv == 0.f && ratio == kPosInf) ratio = 1.f;  // r A is 0 at A = 0 for any r, also one beyond float32
   const float l1 = -ratio * adv, l2 = -fminf(fmaxf(ratio, p.lo), p.hi) * adv;
   PolicyRow o{max_nan(l1, l2), 0.f, l2 > l1 ? 0.f : l1};
   if (p.ref != nullptr) {

@@ -389,6 +389,7 @@ typedef struct dslpg_logit_rows {
  *   g = dloss/dlogp = (0 where the clipped term alone counts, else -r A) + kl_coef (1 - exp(d))
  *   dlogits = dloss g logit_scale (onehot(label) - softmax(z))
  * 0 <= clip_low <= 1, clip_high >= 0. With kl_coef 0 the KL term is only reported.
+ * Where A is 0 there is no policy term, however large r is.
  */
 typedef struct dslpg_policy_terms {
   const float* old_logp;
