@@ -208,10 +208,10 @@ DSLPG_DEV PolicyRow policy_row(const PolicyTerms& p, float old_logp, float adv, 
     const float d = static_cast<float>(static_cast<double>(ref) - logp);
     const float e = expm1f(d);
     // exp(d) - d - 1; its power series near 0, where the difference cancels (|d| < 1/4: the first term left out is
-    // below 2e-8 of the sum)
+    // below 2e-8 of the sum). At d = inf (logp = -inf) it is inf, not inf - inf.
     o.kl = fabsf(d) < 0.25f
                ? d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040))))))
-               : e - d;
+               : (d == kPosInf ? d : e - d);
     if (p.kl_coef != 0.f) {
       o.loss += p.kl_coef * o.kl;
       o.g -= p.kl_coef * e;

@@ -1,8 +1,10 @@
-"""policy_loss at the edges of its formulas: an advantage of 0 with a ratio beyond float32."""
+"""policy_loss at the edges of its formulas: an advantage of 0 with a ratio beyond float32, and a sampled token whose
+logit is masked, with a reference."""
 import pytest
 import torch
 
 import dslperfgap_b200 as B
+from loss_ref import U
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +52,24 @@ def test_zero_advantage_and_ratio_beyond_float32(way, clip_high):
     old[0], adv[1] = float("nan"), -1.0
     loss = B.policy_loss_fwd(x, y, old, adv)[0]
     assert loss[0].isnan() and loss[1] == float("inf")
+
+
+@pytest.mark.parametrize("kl_coef", [0.0, 0.1])
+@pytest.mark.parametrize("way", WAYS)
+def test_masked_sampled_token_with_reference(way, kl_coef):
+    """logp = -inf against a finite reference: exp(d) - d - 1 grows without bound, so kl is infinite, not NaN; the other
+    infinite differences keep their limits."""
+    x, y, logp = rows(way, 5, seed=1)
+    old, ref = logp.float(), (logp + 0.25).float()
+    x[1, y[1]] = float("-inf")
+    ref[2] = float("-inf")
+    inf = float("inf")
+    fwd, both, _, _ = all_ways(x, y, old, torch.ones(5, device="cuda"), torch.ones(5, device="cuda"), ref_logp=ref,
+                               kl_coef=kl_coef)
+    for loss, lp, lse, kl in (fwd, both):
+        assert lp[1] == -inf and kl[1] == inf and kl[2] == inf
+        assert loss[1] == (inf if kl_coef else 0) and (loss[2] == inf if kl_coef else loss[2].isfinite())
+        # d is 1/4, off by half steps of lse, logp and the reference's rounding (sizes below 64) and the sum's 160
+        d = torch.tensor(0.25, dtype=torch.float64, device="cuda")
+        slack = torch.expm1(d) * U * (160 + 4 * 64) + 16 * U
+        assert ((kl[[0, 3, 4]].double() - (torch.expm1(d) - d)).abs() <= slack).all()
