@@ -2,13 +2,12 @@
 ``preference_loss``), and the rows as the C ABI's ``dslpg_logit_rows``."""
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
 
 MAX_COLS = 1 << 30
+MIN_SCALE, MAX_SCALE = 1e-30, 1e30  # the exponents' constant is held in float32
 
 
 def check_rows(logits, labels, logit_scale, what: str) -> None:
@@ -19,8 +18,8 @@ def check_rows(logits, labels, logit_scale, what: str) -> None:
         raise TypeError(f"{what}: labels must be int32 or int64, got {labels.dtype}")
     if labels.dim() != 1 or labels.shape[0] != logits.shape[0]:
         raise ValueError(f"{what}: labels shape {tuple(labels.shape)} != ({logits.shape[0]},)")
-    if not math.isfinite(logit_scale):
-        raise ValueError(f"{what}: logit_scale must be finite, got {logit_scale}")
+    if logit_scale != 0 and not MIN_SCALE <= abs(logit_scale) <= MAX_SCALE:
+        raise ValueError(f"{what}: logit_scale must be 0 or {MIN_SCALE} to {MAX_SCALE} in size, got {logit_scale}")
 
 
 def check_vector(x, n: int, name: str, what: str) -> None:

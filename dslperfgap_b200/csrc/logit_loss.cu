@@ -879,12 +879,15 @@ cudaError_t dispatch(Way way, int dt, const LossRows& a, const PolicyTerms& pol,
 
 bool finite(double v) { return v - v == 0.0; }
 
+// c's first part has to be a normal float32, and its second one (2^-24 of it, or 2^-126 in place of 0) small beside it.
+bool scale_ok(double v) { return v == 0.0 || (fabs(v) >= 1e-30 && fabs(v) <= 1e30); }
+
 int rows_args(LossRows& a, const dslpg_logit_rows* h) {
   if (!h) return DSLPG_ERR_NULL_POINTER;
   if (!is_float_dtype(h->logits_dtype) || (h->labels_dtype != DSLPG_I32 && h->labels_dtype != DSLPG_I64))
     return DSLPG_ERR_BAD_DTYPE;
   if (h->n_rows < 0 || h->n_cols < 1 || h->n_cols > (1ll << 30) || h->row_stride < h->n_cols) return DSLPG_ERR_BAD_SHAPE;
-  if (!finite(h->logit_scale)) return DSLPG_ERR_BAD_ARGUMENT;
+  if (!scale_ok(h->logit_scale)) return DSLPG_ERR_BAD_ARGUMENT;
   if (h->n_rows > 0 && (!h->logits || !h->labels)) return DSLPG_ERR_NULL_POINTER;
   a.x = h->logits;
   a.labels = h->labels;

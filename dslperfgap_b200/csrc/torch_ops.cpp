@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cmath>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -454,7 +455,8 @@ struct LossRows {
     r.logit_scale = scale.cast<double>();
     r.logits_dtype = float_code(x->scalar_type());
     r.labels_dtype = lab->scalar_type() == at::kLong ? DSLPG_I64 : DSLPG_I32;
-    return r.logit_scale - r.logit_scale == 0.0;
+    const double size = std::fabs(r.logit_scale);
+    return size == 0.0 || (size >= 1e-30 && size <= 1e30);
   }
   int dev() const { return logits.get_device(); }
   at::Tensor f32(int64_t n) const { return at::empty({n}, logits.options().dtype(at::kFloat)); }

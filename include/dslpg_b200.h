@@ -370,7 +370,8 @@ DSLPG_API int dslpg_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, con
  * labels [n_rows] (int32 or int64), dense. With z = logit_scale * logits:
  * lse = log sum exp z, logp = z[label] - lse (both float32 outputs [n_rows]).
  * A row whose label is ignored_index, or no column, is left out: its logits are
- * not read, and its loss, logp, lse, kl and gradient are 0. n_cols <= 2^30.
+ * not read, and its loss, logp, lse, kl and gradient are 0. n_cols <= 2^30;
+ * logit_scale is 0, or 1e-30 to 1e30 in size.
  * No reference counterpart: the suite has the cross-entropy of such rows.
  */
 typedef struct dslpg_logit_rows {
