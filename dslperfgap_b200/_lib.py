@@ -223,12 +223,16 @@ def torch_ops():
 
 def fast_op(name: str):
     """Callable taking the wrapper's arguments and returning its result, or
-    None when the C++ fast path does not take the case (or is not built)."""
+    None when the C++ fast path does not take the case (or is not built). With
+    no library at all the wrapper goes on too: its argument checks need none,
+    and its launch raises."""
     state = {}
 
     def call(*args):
         fn = state.get("fn")
         if fn is None:
+            if _lib is None and not LIB_PATH.exists():
+                return None
             mod = torch_ops()
             fn = state["fn"] = getattr(mod, name) if mod is not None else (lambda *a: None)
         return fn(*args)
