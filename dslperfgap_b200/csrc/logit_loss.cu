@@ -844,12 +844,25 @@ cudaError_t launch_fused(LossRows a, const PolicyTerms& pol, const LossOut& o, c
   const int64_t vecs = a.N / E;
   if (vec && vecs <= 2 * 128) return launch_short<T, 2>(a, pol, o, go, st);
   if (vec && vecs <= 8 * 512) return launch_short<T, 8>(a, pol, o, go, st);
-  // rows in flight stay in L2: one CTA of 1024 threads an SM, or several small ones
-  const int64_t most = vecs > 4 * 256 ? sm_count() : 8 * sm_count();
-  const int grid = static_cast<int>(a.M < most ? a.M : most);
-  auto launch = [&](auto small, auto large) {
-    if (vecs > 4 * 256) large<<<grid, 1024, 0, st>>>(a, pol, o, go);
-    else small<<<grid, 128, 0, st>>>(a, pol, o, go);
+  // Both passes in one kernel pay where a CTA has one row (the second launch is saved), and for many long rows, whose
+  // second reading then comes from L2. Elsewhere the forward and the backward kernel follow one another: of many shorter
+  // rows an SM has several in flight there, and of few long ones several SMs share each. One kernel / two, in us, bf16:
+  // [300, 1001] 8.4 / 9.7, [600, 1001] 12.4 / 10.3, [40000, 1001] 851 / 97; [148, 9001] 10.4 / 12.4, [10000, 9001]
+  // 305 / 117; [6000, 48001] 319 / 289, [6000, 64001] 369 / 370, [6000, 96001] 495 / 539, [8192, 128256] 817 / 924;
+  // [8, 2^20] 94 / 21, [74, 128256] 23.4 / 19.9, [100, 128256] 24.7 / 27.3; fp32 [2000, 28001] 124 / 120, [2000, 32001]
+  // 128 / 135, [64, 128256] 37 / 29, [148, 128256] 44 / 57.
+  const bool small = vecs <= 4 * 256, longer = a.N * static_cast<int64_t>(sizeof(T)) >= 112 * 1024;
+  const int64_t sms = sm_count();
+  if (longer ? 2 * a.M <= sms : a.M > (small ? 2 * sms : sms)) {
+    if (cudaError_t e = launch_rows<kPolicy, T>(a, pol, PairTerms{}, o, st)) return e;
+    GradOut from = go;
+    from.lse = o.lse;
+    return launch_bwd<kPolicy, T>(a, pol, PairTerms{}, from, st);
+  }
+  const int grid = static_cast<int>(small || a.M < sms ? a.M : sms);  // one CTA of 1024 threads an SM
+  auto launch = [&](auto few, auto large) {
+    if (small) few<<<grid, 128, 0, st>>>(a, pol, o, go);
+    else large<<<grid, 1024, 0, st>>>(a, pol, o, go);
   };
   if (same_phase<T>(a, go)) launch(&policy_two_pass_kernel<T, 128, true>, &policy_two_pass_kernel<T, 1024, true>);
   else launch(&policy_two_pass_kernel<T, 128, false>, &policy_two_pass_kernel<T, 1024, false>);

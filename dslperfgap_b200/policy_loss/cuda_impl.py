@@ -8,9 +8,9 @@ Per row, with z = logit_scale * logits and logp = z[label] - logsumexp(z)::
 ``policy_loss_fwd`` returns ``(loss, logp, lse, kl)``, float32 ``[n_rows]``
 each; ``policy_loss_bwd`` returns dlogits (the logits' shape and type) from the
 forward's ``lse`` and the losses' gradients ``dloss``; ``policy_loss_fwd_bwd``
-does both with one reading of the logits, for a ``dloss`` known beforehand (the
-weights of a mean over tokens, for instance), and returns ``(loss, logp, lse,
-kl, dlogits)``. The suite has no kernel of this kind; the calling convention is
+does both in one call, with one reading of the logits where their length allows
+it, for a ``dloss`` known beforehand (the weights of a mean over tokens, for
+instance), and returns ``(loss, logp, lse, kl, dlogits)``. The suite has no kernel of this kind; the calling convention is
 cross_entropy's.
 
 ``old_logp``, ``advantages``, ``ref_logp`` and ``dloss`` are float32 ``[n_rows]``

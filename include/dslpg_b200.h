@@ -410,7 +410,8 @@ DSLPG_API int dslpg_policy_loss_bwd(const dslpg_logit_rows* rows, const dslpg_po
                                     int64_t dloss_stride, const float* lse, void* dlogits, int64_t dlogits_row_stride,
                                     cudaStream_t stream);
 
-/* Both in one pass over the logits, for a dloss known beforehand. */
+/* Both in one call, for a dloss known beforehand: the logits are read from HBM
+ * once where their length allows it. */
 DSLPG_API int dslpg_policy_loss_fwd_bwd(const dslpg_logit_rows* rows, const dslpg_policy_terms* terms,
                                         const float* dloss, int64_t dloss_stride, float* loss, float* logp, float* lse,
                                         float* kl, void* dlogits, int64_t dlogits_row_stride, cudaStream_t stream);

@@ -98,3 +98,22 @@ def test_shared_rows_masked_with_the_lowest_value(cols, dt):
     slope = 0.25 * torch.tensor([1.0, -1.0], device="cuda", dtype=torch.float64)[:, None]
     close(dx[:2], slope * want[:2], 160 * L.U * (slope * want[:2]).abs(), "preference grad")
     assert not dx[2:].any()
+
+
+@pytest.mark.parametrize("rows,cols,pad,dt", [(3000, 1001, 0, "bf16"), (2500, 1001, 7, "f16"), (2500, 9001, 0, "f32"),
+                                              (700, 40001, 0, "bf16"), (5, 1 << 20, 8, "bf16"), (40, 128256, 0, "f32")])
+def test_fused_call_of_rows_that_two_kernels_take(rows, cols, pad, dt):
+    """Many rows off the 16-byte boundary, and few long ones, are the forward's and the backward's work one after another
+    (one kernel for both took up to nine times as long): the same bits as the two calls."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x = rn(rows, cols + pad).to(DT[dt])[:, :cols]
+    y = torch.randint(0, cols, (rows,), generator=g, device="cuda")
+    y[1::5] = -100
+    old, adv, dloss, ref = -7 + rn(rows), rn(rows), rn(rows), -7 + rn(rows)
+    how = dict(ref_logp=ref, kl_coef=KL, logit_scale=SCALE)
+    fwd = B.policy_loss_fwd(x, y, old, adv, **how)
+    dx = B.policy_loss_bwd(dloss, x, fwd[2], y, old, adv, **how)
+    both = B.policy_loss_fwd_bwd(x, y, old, adv, dloss, **how)
+    for name, a, b in zip(("loss", "logp", "lse", "kl", "grad"), both, (*fwd, dx)):
+        assert torch.equal(a, b), name
