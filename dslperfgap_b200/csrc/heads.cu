@@ -800,7 +800,7 @@ template <typename T> void set_tiles(HeadArgs& a, int op) {
   const int heads = a.heads[0] + a.heads[1], copies = op == kNormBwd ? 2 : 1, sms = sm_count();
   a.row_bytes = a.D * static_cast<int>(sizeof(T));
   const int64_t row = static_cast<int64_t>(a.row_bytes) * copies, token = row * heads;
-      const int64_t want = (op == kRotate ? 40 : 80) * 1024;
+  const int64_t want = (op == kRotate ? 40 : 80) * 1024;
   a.parts = 1;
   a.part = heads;
   a.tt = 1;

@@ -319,8 +319,9 @@ template <int KIND> DSLPG_DEV int64_t counted_col(const LossRows& a, const PairT
 }
 
 // Row statistics: `tpr` threads a row. HBM-bound: bf16 [6000, 128256] with 1500
-// rows left out takes 188 us (6.14 TB/s of 6.51 measured) with 4 loads in flight a
-// thread and 4 CTAs an SM; 3 CTAs 202, 5 193; 2, 3, 6 and 8 loads 197, 194, 223, 221.
+// rows left out takes 188 us (6.14 TB/s of 6.51 measured) in a loop over one batch,
+// 202 over three in turn, with 4 loads in flight a thread and 4 CTAs an SM; in the
+// loop 3 CTAs 202, 5 193; 2, 3, 6 and 8 loads 197, 194, 223, 221.
 // A CTA a row, handed out by the hardware: shared out evenly beforehand, rows that
 // are left out leave some CTAs with less than others (261 us). Writes the row's losses (policy) or its
 // logp and lse (preferences; pair_kernel then sums them).
@@ -454,8 +455,10 @@ DSLPG_DEV Vec16 shifted_vec(const Vec16& lo, const Vec16& hi, int s) {
 // dlogits of elements [0, n) by `nt` threads, this one being t, then the label
 // column (col, if in there): k1 expm1(logp). Vectors are those of the output; the
 // logits' may lie at another distance from a 16-byte boundary (rows of odd
-// length). The next chunk's loads are issued before this chunk's arithmetic.
-// SAME: they lie at the same one in every row.
+// length). Where they lie at the same one (SAME: in every row), the next chunk's
+// loads are issued before this chunk's arithmetic; elsewhere two vectors are read
+// for each one written, two at a time, with nothing ahead (126 registers already):
+// fp16 [2048, 32001] in rows 32064 apart 81 us, [2048, 32000] 50.
 template <typename T, int U, bool SAME, bool FAR>
 DSLPG_DEV void grad_row_as(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
   constexpr int E = Elt<T>::kPerVec;
@@ -528,6 +531,8 @@ DSLPG_DEV void grad_row_as(const T* xr, T* yr, int64_t n, const GradTerms& gt, d
   }
 }
 
+// (`far`: one vector at a time, to keep the registers of the other loop. It begins at |lse| of 44 and costs: bf16
+// [4096, 128256] with lse near 60 448 us, near 16 316.)
 template <typename T, int U, bool SAME>
 DSLPG_DEV void grad_row(const T* xr, T* yr, int64_t n, const GradTerms& gt, double logp, int64_t col, int t, int nt) {
   if (gt.far) grad_row_as<T, 1, SAME, true>(xr, yr, n, gt, logp, col, t, nt);
@@ -620,8 +625,9 @@ __global__ void __launch_bounds__(256) loss_bwd_kernel(const __grid_constant__ L
 }
 
 // Loss and gradient in one kernel, any row: a CTA a row, whose second reading
-// comes from L2 (the rows in flight, one an SM, are a third of it; the first
-// reading marks its lines to stay). Rows are taken NT at a time: of the counted
+// comes from L2 while the rows in flight, one an SM, fit there (38 MB for 16-bit
+// rows of 128256, 76 MB in fp32; the first reading marks its lines to stay, and
+// nothing demotes them). Rows are taken NT at a time: of the counted
 // ones among them, and of the left-out ones, CTA k does every G-th by their
 // number, so that none gets more of either kind than another.
 // Bound by instructions and latency: one pass of a row at a time is on an SM, so its
@@ -709,8 +715,9 @@ __global__ void __launch_bounds__(NT, 1) policy_two_pass_kernel(const __grid_con
   }
 }
 
-// Loss and gradient of rows that the registers of their threads hold (NV vectors
-// a thread, 16-byte rows): read once, written once.
+// Loss and gradient of rows that their threads hold (NV vectors a thread, 16-byte
+// rows): read once, written once. In registers, but for 8 vectors of fp32, of which
+// 128 bytes lie in local memory ([2048, 8192] 37.8 us of a floor of 19.6).
 template <typename T, int NV>
 __global__ void __launch_bounds__(512) policy_short_kernel(const __grid_constant__ LossRows a,
                                                            const __grid_constant__ PolicyTerms pol, const LossOut o,
